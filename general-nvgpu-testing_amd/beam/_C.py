@@ -11,6 +11,7 @@ code of the library becomes a BeamError.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -103,6 +104,10 @@ def _load() -> ctypes.CDLL:
     L.beam_parallel_gemmrc_silu.argtypes = [vp, vp, vp, i, i, i, vp, vp, ctypes.c_longlong, i, cfgp, vp]
     L.beam_silu.argtypes = [vp, vp, ctypes.c_longlong, i, vp]
     L.beam_matmul_nn.argtypes = [vp, vp, vp, i, i, i, i, cfgp, vp]
+    L.beam_gemmrc_gated.argtypes = [vp, vp, vp, vp, i, i, i, i, vp]
+    L.beam_gemmrc_gated_backward_workspace_bytes.argtypes = [i, i, i, i]
+    L.beam_gemmrc_gated_backward_workspace_bytes.restype = sz
+    L.beam_gemmrc_gated_backward.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
     L.beam_bench.argtypes = [i, ctypes.POINTER(_Problem), cfgp, i, i, vp, ctypes.POINTER(ctypes.c_float)]
     L.beam_stream_create.argtypes = [ctypes.POINTER(vp)]
     L.beam_stream_destroy.argtypes = [vp]
@@ -129,6 +134,7 @@ def _load() -> ctypes.CDLL:
     L.beam_dbg_ln_plan_bytes.restype = sz
     L.beam_dbg_assume_compute_units.argtypes = [i]
     L.beam_dbg_small_tile.argtypes = [i, i, i, i, i] + [ctypes.POINTER(i)] * 4
+    L.beam_dbg_gated_tile.argtypes = [i, i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_nn_off_lines_tile.argtypes = [i, i, i, cfgp, cfgp, ctypes.POINTER(i)]
     L.beam_dbg_off_lines_tile.argtypes = L.beam_dbg_ln_line_tile.argtypes = [i, i, i, cfgp, ctypes.POINTER(i)]
     L.beam_set_ln_walk.argtypes = [i]
@@ -565,6 +571,86 @@ def parallel_gemmrc_silu(a, b, c, x, y, config: Optional[TileConfig] = None) -> 
     px, py, n, _, _ = _flat_pair(x, y, d)
     cfg = config.to_c() if config is not None else None
     _check(lib.beam_parallel_gemmrc_silu(pa, pb, pc, M, N, K, px, py, n, d, ctypes.byref(cfg) if cfg else None, st))
+
+
+# ---------------------------------------------------------------------------- gated layer
+
+
+def _same_device(*xs):
+    """Raises unless the torch tensors among xs lie on one GPU; a context in which that GPU is the current one."""
+    device = None
+    for x in xs:
+        if _Tensor is not None and isinstance(x, _Tensor):
+            if not x.is_cuda:
+                raise BeamError(1, "tensor is not on the GPU")
+            if device is not None and x.device != device:
+                raise BeamError(1, f"tensors on {device} and {x.device}")
+            device = x.device
+    return _here if device is None or device.index == _torch.cuda.current_device() else _torch.cuda.device(device)
+
+
+_here = contextlib.nullcontext()
+_scratch: Optional[DeviceArray] = None  # for calls on DeviceArrays: they all go to the default stream, one after the other
+
+
+def _call_workspace(like, nbytes: int):
+    """(pointer, what keeps it) of workspace for one call: for tensors from torch's allocator, which knows streams and captures,
+    so that no other stream's call and no other graph has the same bytes while this one runs."""
+    global _scratch
+    if nbytes == 0:
+        return None, None
+    if _Tensor is not None and isinstance(like, _Tensor):
+        t = _torch.empty(nbytes, device=like.device, dtype=_torch.uint8)
+        return t.data_ptr(), t
+    if _scratch is None or _scratch.nbytes < nbytes:
+        if _scratch is not None:
+            _check(lib.beam_sync(None))
+            _scratch.free()
+        _scratch = DeviceArray((max(nbytes, 1 << 20),), itemsize=1)
+    return _scratch.ptr, _scratch
+
+
+def _matrix(x, name: str, rows: Optional[int] = None, cols: Optional[int] = None, dtype: Optional[int] = None):
+    p, s, d = _describe(x)
+    if len(s) != 2:
+        raise BeamError(1, f"{name} must be 2-D")
+    if (rows is not None and s[0] != rows) or (cols is not None and s[1] != cols):
+        raise BeamError(1, f"{name} has shape {tuple(s)}, expected {(s[0] if rows is None else rows, s[1] if cols is None else cols)}")
+    if max(s) > 0x7FFFFFFF:
+        raise BeamError(2, f"{name} has shape {tuple(s)}: too large")
+    if dtype is not None and d != dtype:
+        raise BeamError(2, f"{name} must be {_DTYPE_NAMES[dtype]} as the first operand")
+    return p, s[0], s[1], d
+
+
+def gemmrc_gated(a, b, h, gu=None) -> None:
+    """h = silu(a @ b[:N].T) * (a @ b[N:].T) in one launch: a [M, K], b [2 N, K] (the gate's rows, then the other projection's),
+    h [M, N].  gu [M, 2 N], if given, gets the two factors before the activation, what gemmrc_gated_backward takes."""
+    with _same_device(a, b, h, gu):
+        pa, M, K, d = _matrix(a, "a")
+        pb, N2, _, _ = _matrix(b, "b", None, K, d)
+        if N2 % 2:
+            raise BeamError(1, f"b has {N2} rows; it holds two projections of as many rows each")
+        ph = _matrix(h, "h", M, N2 // 2, d)[0]
+        pg = _matrix(gu, "gu", M, N2, d)[0] if gu is not None else None
+        _check(lib.beam_gemmrc_gated(pa, pb, ph, pg, M, N2 // 2, K, d, _stream_of(a)))
+
+
+def gemmrc_gated_backward(dh, gu, a, b, da=None, db=None) -> None:
+    """The gradients of gemmrc_gated: dh [M, N] is h's, gu [M, 2 N] what the forward call wrote; da [M, K] and db [2 N, K] are
+    written, either may be left out."""
+    with _same_device(dh, gu, a, b, da, db):
+        pa, M, K, d = _matrix(a, "a")
+        pb, N2, _, _ = _matrix(b, "b", None, K, d)
+        if N2 % 2:
+            raise BeamError(1, f"b has {N2} rows; it holds two projections of as many rows each")
+        pdh, pgu = _matrix(dh, "dh", M, N2 // 2, d)[0], _matrix(gu, "gu", M, N2, d)[0]
+        pda = _matrix(da, "da", M, K, d)[0] if da is not None else None
+        pdb = _matrix(db, "db", N2, K, d)[0] if db is not None else None
+        need = lib.beam_gemmrc_gated_backward_workspace_bytes(M, N2 // 2, da is not None, db is not None)
+        ws, keep = _call_workspace(a, need)
+        _check(lib.beam_gemmrc_gated_backward(pdh, pgu, pa, pb, pda, pdb, M, N2 // 2, K, d, ws, need, _stream_of(a)))
+        del keep
 
 
 def _fixed(fn_name: str):

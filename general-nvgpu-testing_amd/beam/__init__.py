@@ -17,6 +17,8 @@ from ._C import (  # noqa: F401
     cutlass_parallel_gemmrc_lnr,
     device_info,
     gemmrc,
+    gemmrc_gated,
+    gemmrc_gated_backward,
     gemmrc_ln,
     gemmrc_spec,
     gemmrc_splitk,

@@ -18,6 +18,7 @@
 
 #include "../../include/beam_hip_debug.h"
 #include "aux_kernels.h"
+#include "gated.h"
 #include "kernel_set.h"
 #include "tile_map.h"
 
@@ -992,6 +993,121 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
   return BEAM_OK;
 }
 
+// ---- gated layer ------------------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+// The tile of gemm_kwave.h for a gated layer, if any; as kw_plan for its 2 N rows of B, of which the tiles here have 32 or 64.
+KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
+  static const struct { int rows, cols; } kTiles[] = {{8, 32}, {16, 32}, {32, 32}, {8, 64}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
+  const KwPlan none = {0, 0, 0, false};
+  if (K < 8 || K > kMaxK) return none;
+  for (const auto& t : kTiles) {
+    if (t.rows == 8 && M > 8) continue;
+    const long tiles = ((long)M + t.rows - 1) / t.rows * (((long)N + t.cols / 2 - 1) / (t.cols / 2));
+    // a handful of rows: B is read once whatever the number of tiles
+    const bool few = M <= 16 && t.rows >= M && t.cols == 64;
+    if (tiles > cus && !few) continue;
+    const bool shift = rows == kOnChunks && t.rows > 8 && !(M <= 16 && t.cols == 64) && (long)(K / kBK) * (t.rows + t.cols) >= 1200;
+    if (t.rows * t.cols == 64 * 64 && (rows == kOnLines ? K >= 2048 : shift)) return none;
+    return KwPlan{t.rows, t.cols, 4, shift};
+  }
+  return none;
+}
+
+// The tile of the gated kernel: what beam_gemmrc would take for the 2 N rows of B, as far as there is one like it.
+GatedTile gated_tile(int M, int N, int K, RowStarts rows, int cus) {
+  if (K % kBK != 0 && rows == kOnChunks) {
+    const LineChoice t = off_lines_tile(M, 2 * N, K, cus);
+    if (t.lines) return GatedTile{t.cfg.block_m == 128 && t.cfg.block_n == 64 ? 64 : t.cfg.block_m, 128, kGatedLines};
+  }
+  beam_tile_cfg c;
+  int s;
+  (void)choose_default(M, 2 * N, K, -1, &c, &s);
+  if (c.block_m * c.block_n <= 128 * 64) return GatedTile{64, 128, c.pipeline == 2 ? kGatedDeep : kGatedShallow};
+  return GatedTile{c.block_m, c.block_n, c.pipeline == 2 && c.block_m * c.block_n == 128 * 128 ? kGatedDeep : kGatedShallow};
+}
+
+// A [M][K] and the layer's 2 N rows of B: what every entry refuses.
+int check_gated(const void* A, const void* B, const void* H, int M, int N, int K, int dtype, bool* generic) {
+  if (N > INT32_MAX / 4) return fail(BEAM_ERR_UNSUPPORTED, "N=%d too large", N);
+  return check_problem(A, B, H, M, N, K, dtype, generic);
+}
+
+}  // namespace
+
+extern "C" {
+
+int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, void* stream) {
+  bool generic;
+  int rc = check_gated(A, B, H, M, N, K, dtype, &generic);
+  if (rc) return rc;
+  if ((uintptr_t)GU & 1) return fail(BEAM_ERR_INVALID, "GU must be aligned to its 16-bit elements");
+  if (M == 0 || N == 0) return BEAM_OK;
+  if ((rc = beam_init())) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (K == 0) {
+    BEAM_HIP(launch_zero_u16(H, (size_t)M * N, st));
+    if (GU) BEAM_HIP(launch_zero_u16(GU, (size_t)M * 2 * N, st));
+    return BEAM_OK;
+  }
+  if (generic) {
+    BEAM_HIP(launch_gated_plain(A, B, H, GU, M, N, K, dtype, st));
+    return BEAM_OK;
+  }
+  const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
+  const RowStarts rows = row_starts(A, B, K, false);
+  if (const KwPlan kw = gated_kw_plan(M, N, K, rows, cus); kw.rows) {
+    KwGatedParams p;
+    KwPlan half = kw;
+    half.cols /= 2;
+    kw_params(&p, half, A, B, H, M, N, K);
+    p.gu = GU;
+    BEAM_HIP(dtype == BEAM_F16 ? launch_gated_kwave<_Float16>(kw, p, st) : launch_gated_kwave<__bf16>(kw, p, st));
+    return BEAM_OK;
+  }
+  const GatedTile t = gated_tile(M, N, K, rows, cus);
+  const beam_tile_cfg c = {t.block_m, t.block_n / 2, 0, 0, 0, default_group_m(t.block_m, t.block_n)};
+  GemmParams p = base_params(A, B, M, N, K, c);
+  p.C = H;
+  p.gu = GU;
+  p.c_store = store_kind(c, 0, false, H, M, N, K);
+  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, 1);
+  BEAM_HIP(dtype == BEAM_F16 ? launch_gated<_Float16>(t, p, grid, st) : launch_gated<__bf16>(t, p, grid, st));
+  return BEAM_OK;
+}
+
+size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int want_dA, int want_dB) {
+  if (M <= 0 || N <= 0) return 0;
+  const size_t one = align_up((size_t)M * 2 * N * 2, 256);
+  return (want_dA ? one : 0) + (want_dB ? one : 0);
+}
+
+int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
+                               int dtype, void* ws, size_t ws_bytes, void* stream) {
+  if (!dA && !dB) return BEAM_OK;
+  bool generic;
+  int rc = check_gated(A, B, dA ? dA : dB, M, N, K, dtype, &generic);
+  if (rc) return rc;
+  if (((uintptr_t)dH | (uintptr_t)GU | (uintptr_t)dA | (uintptr_t)dB) & 1) return fail(BEAM_ERR_INVALID, "operands must be aligned to their 16-bit elements");
+  if (K == 0) return BEAM_OK;
+  if ((size_t)((M + 63) / 64) * ((N + 63) / 64) > INT32_MAX) return fail(BEAM_ERR_UNSUPPORTED, "M=%d x N=%d too large", M, N);
+  if (dB && (2 * N + 63) / 64 > 65535) return fail(BEAM_ERR_UNSUPPORTED, "N=%d too large for dB", N);
+  if (M > 0 && N > 0 && (!dH || !GU)) return fail(BEAM_ERR_INVALID, "null input pointer");
+  const size_t need = beam_gemmrc_gated_backward_workspace_bytes(M, N, dA != nullptr, dB != nullptr);
+  if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255) != 0))
+    return fail(BEAM_ERR_WORKSPACE, "workspace of %zu bytes on 256 needed, %zu given", need, ws ? ws_bytes : (size_t)0);
+  if ((rc = beam_init())) return rc;
+  char* const d = (char*)ws;
+  char* const dt = d + (dA ? align_up((size_t)M * 2 * N * 2, 256) : 0);
+  if (M > 0 && N > 0) BEAM_HIP(launch_gated_gradients(dH, GU, dA ? d : nullptr, dB ? dt : nullptr, M, N, dtype, (hipStream_t)stream));
+  if (dA && (rc = beam_matmul_nn(d, B, dA, M, K, 2 * N, dtype, nullptr, stream))) return rc;
+  if (dB && (rc = beam_matmul_nn(dt, A, dB, 2 * N, K, M, dtype, nullptr, stream))) return rc;
+  return BEAM_OK;
+}
+
 int beam_silu(const void* X, void* Y, long long count, int dtype, void* stream) {
   if (count < 0) return fail(BEAM_ERR_INVALID, "negative element count %lld", count);
   if (dtype != BEAM_F16 && dtype != BEAM_BF16) return fail(BEAM_ERR_UNSUPPORTED, "dtype %d: only fp16 (0) and bf16 (1)", dtype);
@@ -1789,6 +1905,18 @@ int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, 
   *cols = kw.cols;
   *waves = kw.waves;
   *whole_lines = kw.shift ? 1 : 0;
+  return BEAM_OK;
+}
+
+int beam_dbg_gated_tile(int M, int N, int K, int row_starts, int* rows, int* cols, int* kind) {
+  if (!rows || !cols || !kind || row_starts < 0 || row_starts > 2) return fail(BEAM_ERR_INVALID, "arguments");
+  const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
+  if (const KwPlan kw = gated_kw_plan(M, N, K, (RowStarts)row_starts, cus); kw.rows) {
+    *rows = kw.rows, *cols = kw.cols, *kind = kw.shift ? 5 : 4;
+    return BEAM_OK;
+  }
+  const GatedTile t = gated_tile(M, N, K, (RowStarts)row_starts, cus);
+  *rows = t.block_m, *cols = t.block_n, *kind = t.depth;
   return BEAM_OK;
 }
 

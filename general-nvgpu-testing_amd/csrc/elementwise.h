@@ -33,6 +33,14 @@ __device__ __forceinline__ float silu_f32(float x) {
   return r;
 }
 
+// silu(gate) * up of a gated layer, before its rounding to T.
+template <typename T>
+__device__ __forceinline__ float gated_f32(float gate, float up) {
+  float r = silu_f32<!__is_same(T, _Float16)>(gate) * up;
+  asm("" : "+v"(r));  // (a plain multiply, as in silu_f32)
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ T silu_16(T x) {
   return (T)silu_f32<sizeof(T) == 2 && !__is_same(T, _Float16)>((float)x);

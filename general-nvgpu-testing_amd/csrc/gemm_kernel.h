@@ -99,6 +99,10 @@ enum Epilogue : int {
   // through to memory, followed in the same grid by reducing workgroups that add the slices of a tile in
   // slice order as soon as all of them have signalled (splitk_reduce_part_of below).
   kEpiPartialFused = 7,
+  // Gated layer (own launchers, gated_inst.h): B is [2 N][K], N gate rows in front of N up rows; C = silu(A . gate^T) * (A . up^T).
+  // The 16-column blocks of a tile of B are gate and up rows in turn, so that the two factors of an output are in two
+  // accumulators of one lane; a tile is BN / 2 columns of C.
+  kEpiGated = 8,
 };
 constexpr int kNumEpilogues = 6;  // epilogues of the launch tables
 
@@ -149,6 +153,7 @@ struct GemmParams {
   // kEpiPartialFused, measurement only: 1 = no reducing workgroups; the multiplying workgroup of (tile, slice s)
   // reduces parts s, s + splits, ... of its tile itself.  Every multiplying workgroup must then be resident at once.
   int sk_self;
+  void* gu;  // kEpiGated: 16-bit [M][2 N], the two factors before the activation; null: not asked for
 };
 
 // ---- statistics exchange of the fused GEMM+LayerNorm (GemmParams here and in gemm_w4.h, KwLnParams in gemm_kwave.h) ----
@@ -402,6 +407,10 @@ struct GemmTile {
   // wavefront; the fills a tile waits for were issued min(AST, BST) - 1 tiles earlier.
   static constexpr bool SIDE = (EPI == kEpiStoreSide);
   static constexpr bool LOOP = (EPI == kEpiStoreLoop);
+  static constexpr bool GATED = (EPI == kEpiGated);
+  static constexpr int CN = GATED ? BN / 2 : BN;  // columns of C in a tile
+  static constexpr int SN = GATED ? TN / 2 : TN;  // ... and in a wavefront's part of it
+  static constexpr int SFN = SN / 16;
   // global stores of one wavefront per tile when its output leaves as whole rows, 16 bytes per lane
   static constexpr int NST = TM * (TN / 8) / 64;
   static constexpr int SV = HALVES ? 1 : NW / LDW;  // side vectors per loader thread per K tile
@@ -420,7 +429,13 @@ struct GemmTile {
   static_assert(!LINES || NTL % 128 == 0, "whole lines: the rows of a thread's fills lie a multiple of 16 apart");
   static_assert(!LINES || (AST >= 3 && BST >= 3 && !SIDE && !LOOP && (!B_KMAJOR || AST == BST + 1)), "whole lines");
   static_assert(WAIT_STEADY < 64, "vmcnt range");
+  static_assert(!GATED || (!B_KMAJOR && FN % 2 == 0 && LDW % 4 == 0), "a loader's rows of B are all gate or all up rows");
   static_assert(BM * 8 * (4 * WAVES_N + 2) <= LDS_BYTES, "row statistics scratch of the LayerNorm epilogues");
+
+  // Row of a tile of B in LDS -> row of its matrix, from the tile's first one (kEpiGated: of the gate's or the up rows, whichever
+  // the row's block of 16 holds; two loaders in turn have the one kind, two the other).
+  static __device__ __forceinline__ int b_row(int n) { return GATED ? ((n >> 5) << 4) + (n & 15) : n; }
+  static __device__ __forceinline__ bool up_rows(int loader_wave) { return GATED && ((loader_wave >> 1) & 1) != 0; }
 
   // Chunk q = i * NTL + tid of an operand tile lives at LDS byte q * 16 of its slot, which is
   // row q / 8, position q % 8; the position holds logical chunk position ^ swizzle_of_row(row).
@@ -560,7 +575,7 @@ struct GemmTile {
       tc = tile_of_workgroup(blockIdx.x, p.tiles_m, p.tiles_n, p.group_m, p.divs);
     }
     int row0 = tc.tm * BM;
-    int col0 = tc.tn * BN;
+    int col0 = tc.tn * CN;
     const int M = p.M, N = p.N, K = p.K;
 
     // K range of this slice.
@@ -590,11 +605,12 @@ struct GemmTile {
     // Buffer descriptors cover exactly the rows of this tile that exist and the K range of
     // this slice; anything else is out of range: reads return zero and touch no memory.
     int rows_a = (M - row0) < BM ? (M - row0) : BM;
-    int rows_b = (N - col0) < BN ? (N - col0) : BN;
+    int rows_b = (N - col0) < CN ? (N - col0) : CN;
+    const size_t b_row0 = (size_t)col0 + (up_rows(lwave) ? (size_t)N : 0);
     const T* a_base = (const T*)p.A + ((size_t)row0 * K + kb);
     // B as [N][K] (rows of K): like A.  B as [K][N] (B_KMAJOR): the tile's columns start at col0 of
     // row kb; a descriptor is made per K tile (load_b) so that it ends with the tile's last row.
-    const T* b_base = B_KMAJOR ? (const T*)p.B + ((size_t)kb * N + col0) : (const T*)p.B + ((size_t)col0 * K + kb);
+    const T* b_base = B_KMAJOR ? (const T*)p.B + ((size_t)kb * N + col0) : (const T*)p.B + (b_row0 * K + kb);
     unsigned bytes_a = klen > 0 ? ((unsigned)(rows_a - 1) * K + klen) * 2u : 0u;  // (whole lines: chunks behind klen are masked)
     unsigned bytes_b = klen > 0 ? ((unsigned)(rows_b - 1) * K + klen) * 2u : 0u;
     // kEpiStoreLoop: the same for the next tile of this workgroup (neither split-K nor the [K][N]
@@ -624,13 +640,13 @@ struct GemmTile {
     Range range_a{0, 0}, range_b{0, 0};
     // (Offsets count from a line in front of the rows, so that none is negative; rows that do not exist are out of range by
     // their own offset.)
-    auto lines_setup = [&](const T* base, int rows, unsigned* voff, int loads) __attribute__((always_inline)) -> Range {
+    auto lines_setup = [&](const T* base, int rows, unsigned* voff, int loads, auto row_of) __attribute__((always_inline)) -> Range {
       const int r = ltid >> 3;
       const int c = (ltid & 7) ^ swizzle_of_row(r);
-      const int late = c + phase_of(base, r) >= 8 ? 1 : 0;
+      const int late = c + phase_of(base, row_of(r)) >= 8 ? 1 : 0;
 #pragma unroll
       for (int i = 0; i < loads; ++i) {
-        const int row = r + i * (NTL / 8);
+        const int row = row_of(r + i * (NTL / 8));
         voff[i] = row < rows ? (unsigned)kRowBytes + (unsigned)row * (unsigned)K * 2u + (unsigned)(c - 8 * late) * 16u : kOobOffset;
       }
       const int left = (klen >> 3) - 8 * k_first - c;  // chunks from this one on, to the end of K
@@ -638,8 +654,8 @@ struct GemmTile {
       return Range{late, (unsigned)(cnt < n_tiles ? cnt : n_tiles)};
     };
     if constexpr (LINES) {
-      range_a = lines_setup(a_base, rows_a, voff_a, LA);
-      if constexpr (!B_KMAJOR) range_b = lines_setup(b_base, rows_b, voff_b, LB);
+      range_a = lines_setup(a_base, rows_a, voff_a, LA, [](int n) { return n; });
+      if constexpr (!B_KMAJOR) range_b = lines_setup(b_base, rows_b, voff_b, LB, [](int n) { return b_row(n); });
     }
 #pragma unroll
     for (int i = 0; i < (LINES ? 0 : LA); ++i) voff_a[i] = chunk_voffset(i * NTL + ltid, K);
@@ -652,6 +668,9 @@ struct GemmTile {
         const int k = q / CPR;
         const int chunk = (q % CPR) ^ kmajor_swizzle(k, BN);
         voff_b[i] = ((unsigned)k * (unsigned)N + (unsigned)chunk * 8u) * 2u;
+      } else if constexpr (GATED) {
+        const int q = i * NTL + ltid;
+        voff_b[i] = (unsigned)b_row(q >> 3) * (unsigned)K * 2u + (unsigned)((q & 7) ^ swizzle_of_row(q >> 3)) * 16u;
       } else {
         voff_b[i] = chunk_voffset(i * NTL + ltid, K);
       }
@@ -737,7 +756,7 @@ struct GemmTile {
       const int kend = koff + kvalid;      // the row's end in this slice
       const int r = kvalid & 7;            // elements of the chunk that K ends inside
       // rows of A or B ([N][K]) from their own start, so that the shifted chunk's offset is never negative
-      auto load_rows = [&](const void* base, int rows, auto n_tag, i32x4* regs) __attribute__((always_inline)) {
+      auto load_rows = [&](const void* base, int rows, auto n_tag, i32x4* regs, auto row_of) __attribute__((always_inline)) {
         constexpr int L = decltype(n_tag)::value;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(base, ((unsigned)(rows - 1) * (unsigned)K + (unsigned)kend) * 2u);
 #pragma unroll
@@ -745,7 +764,7 @@ struct GemmTile {
           const int q = i * NTL + tid;
           const int c8 = ((q & 7) ^ swizzle_of_row(q >> 3)) * 8;
           const int at = c8 + 8 <= kvalid ? koff + c8 : kend - 8;
-          const unsigned off = c8 < kvalid ? ((unsigned)(q >> 3) * (unsigned)K + (unsigned)at) * 2u : kOobOffset;
+          const unsigned off = c8 < kvalid ? ((unsigned)row_of(q >> 3) * (unsigned)K + (unsigned)at) * 2u : kOobOffset;
           regs[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0);
         }
         if (r != 0) {  // (uniform)
@@ -757,9 +776,9 @@ struct GemmTile {
           }
         }
       };
-      load_rows((const T*)p.A + (size_t)row0 * K, rows_a, std::integral_constant<int, LA>{}, st.a);
+      load_rows((const T*)p.A + (size_t)row0 * K, rows_a, std::integral_constant<int, LA>{}, st.a, [](int n) { return n; });
       if constexpr (!B_KMAJOR) {
-        load_rows((const T*)p.B + (size_t)col0 * K, rows_b, std::integral_constant<int, LB>{}, st.b);
+        load_rows((const T*)p.B + b_row0 * K, rows_b, std::integral_constant<int, LB>{}, st.b, [](int n) { return b_row(n); });
       } else if (n_odd) {
         constexpr int CPR = BN / 8;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc((const T*)p.B + (size_t)koff * N, (unsigned)kvalid * (unsigned)N * 2u);
@@ -792,11 +811,13 @@ struct GemmTile {
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk) frag_off[kk] = lds_offset(lane & 15, 4 * (HALVES ? kg : kk) + (lane >> 4));  // HALVES: the group's half
     // whole lines: the lanes whose chunk of a K tile arrives with the fill behind that tile's own
-    bool late_a[KSTEPS], late_b[KSTEPS];
+    bool late_a[KSTEPS], late_b[KSTEPS], late_up[KSTEPS];
+    const T* const b_first = GATED ? (const T*)p.B + ((size_t)col0 * K + kb) : b_base;
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk) {
       late_a[kk] = LINES && 4 * (HALVES ? kg : kk) + (lane >> 4) + phase_of(a_base, lane & 15) >= 8;
-      late_b[kk] = LINES && !B_KMAJOR && 4 * (HALVES ? kg : kk) + (lane >> 4) + phase_of(b_base, lane & 15) >= 8;
+      late_b[kk] = LINES && !B_KMAJOR && 4 * (HALVES ? kg : kk) + (lane >> 4) + phase_of(b_first, lane & 15) >= 8;
+      late_up[kk] = LINES && GATED && 4 * (HALVES ? kg : kk) + (lane >> 4) + phase_of(b_first + (size_t)N * K, lane & 15) >= 8;
     }
     const int a_wave_off = wm * TM * kRowBytes;
     const int b_wave_off = B_KMAJOR ? 0 : wn * TN * kRowBytes;
@@ -934,7 +955,7 @@ struct GemmTile {
     // left alone, the compiler sinks the reads to the end of the step and re-uses fragment
     // registers across the two sets, and the step then starts by waiting for its own reads.
     //   ROW0: index of the step's first row inside the tile (the loads are dealt out row by row).
-    auto step = [&](const char* sa, const char* sb, vec8(&fa_cur)[FM], vec8(&fa_nxt)[FM], vec8(&fb_cur)[FN],
+    auto step = [&](const char* sa, const char* sb, const char* sb_up, vec8(&fa_cur)[FM], vec8(&fa_nxt)[FM], vec8(&fb_cur)[FN],
                     vec8(&fb_nxt)[FN], int h, auto row0_tag, auto ld_tag, auto w_tag) __attribute__((always_inline)) {
       constexpr int ROW0 = decltype(row0_tag)::value;
       constexpr bool LD = decltype(ld_tag)::value;
@@ -948,7 +969,7 @@ struct GemmTile {
         for (int u = 0; u < PER_READ_ROW; ++u) {
           const int r = i * PER_READ_ROW + u;
           if (i < READ_ROWS && r < READS) {
-            if (r < FN) fb_nxt[r] = read_b_fragment(sb, r);
+            if (r < FN) fb_nxt[r] = read_b_fragment(LINES && GATED && (r & 1) ? sb_up : sb, r);
             else fa_nxt[r - FN] = *(const vec8*)(sa + (r - FN) * 16 * kRowBytes);
           }
         }
@@ -1040,13 +1061,17 @@ struct GemmTile {
         if constexpr (LINES && !B_KMAJOR) return smem + (B_REGION + (late_b[kk] ? ((h + 1) % BST) * B_BYTES : (h % BST) * B_BYTES)) + (b_wave_off + frag_off[kk]);
         return sb + (B_KMAJOR ? (HALVES ? kg : kk) * (32 * BN * 2) : frag_off[kk]);
       };
+      auto up_at = [&](int kk) __attribute__((always_inline)) -> const char* {  // kEpiGated: the same of the blocks of up rows
+        if constexpr (LINES && GATED) return smem + (B_REGION + (late_up[kk] ? ((h + 1) % BST) * B_BYTES : (h % BST) * B_BYTES)) + (b_wave_off + frag_off[kk]);
+        return nullptr;
+      };
       if constexpr (HALVES) {
         // this group's half of tile h is read while its half of tile h - 1 is multiplied
-        if constexpr (decltype(par_tag)::value == 0) step(a_at(0), b_at(0), fa1, fa0, fb1, fb0, h, std::integral_constant<int, 0>{}, ld_tag, w_tag);
-        else step(a_at(0), b_at(0), fa0, fa1, fb0, fb1, h, std::integral_constant<int, 0>{}, ld_tag, w_tag);
+        if constexpr (decltype(par_tag)::value == 0) step(a_at(0), b_at(0), up_at(0), fa1, fa0, fb1, fb0, h, std::integral_constant<int, 0>{}, ld_tag, w_tag);
+        else step(a_at(0), b_at(0), up_at(0), fa0, fa1, fb0, fb1, h, std::integral_constant<int, 0>{}, ld_tag, w_tag);
       } else {
-        step(a_at(0), b_at(0), fa1, fa0, fb1, fb0, h, std::integral_constant<int, 0>{}, ld_tag, w_tag);
-        step(a_at(1), b_at(1), fa0, fa1, fb0, fb1, h, std::integral_constant<int, FM>{}, ld_tag, w_tag);
+        step(a_at(0), b_at(0), up_at(0), fa1, fa0, fb1, fb0, h, std::integral_constant<int, 0>{}, ld_tag, w_tag);
+        step(a_at(1), b_at(1), up_at(1), fa0, fa1, fb0, fb1, h, std::integral_constant<int, FM>{}, ld_tag, w_tag);
       }
       if constexpr (SIDE && decltype(ld_tag)::value) {
         side_store(h, w_tag);
@@ -1326,16 +1351,16 @@ struct GemmTile {
     // XORed with the row number (3 bits; 2 bits and the row's parity where two rows share a
     // window) and rows 8..15 of a block have the two halves of every chunk swapped.  The 16-byte
     // reads run over whole rows (any padding of the rows makes them conflict) and undo both.
-    //   row_ctx(i): per-row values of block row i, passed on to value(i, j, ctx) -> 4 outputs.
-    auto staged_store = [&](T* C, auto reserved_tag, auto row_ctx, auto value) {
+    //   row_ctx(i): per-row values of block row i, passed on to value(i, j, ctx) -> 4 outputs.  ld: elements from a row of C to the next.
+    auto staged_store = [&](T* C, int ld, auto reserved_tag, auto row_ctx, auto value) {
       constexpr int RESERVED = decltype(reserved_tag)::value;
       constexpr int AVAIL = LDS_BYTES - RESERVED;
-      constexpr int RB = TN * 2;  // bytes per row
+      constexpr int RB = SN * 2;  // bytes per row
       constexpr int HALVES = NW * TM * RB <= AVAIL ? 1 : (NW * TM * RB <= 2 * AVAIL ? 2 : 4);
       static_assert(NW * (TM / HALVES) * RB <= AVAIL && FM % HALVES == 0 && RESERVED % 128 == 0, "staging area");
       static_assert(RB == 64 || RB == 128 || RB == 256, "row of a wavefront's sub-tile");
       constexpr int FMH = FM / HALVES;  // blocks of 16 rows per pass
-      constexpr int LPR = TN / 8;       // lanes per row
+      constexpr int LPR = SN / 8;       // lanes per row
       constexpr int RPI = 64 / LPR;     // rows per store instruction
       auto chunk_xor = [](int r) { return RB == 64 ? (r >> 1) & 3 : r & 7; };
       char* stage = smem + RESERVED + wave * (FMH * 16 * RB);
@@ -1348,14 +1373,14 @@ struct GemmTile {
         for (int i = 0; i < FMH; ++i) {
           const auto ctx = row_ctx(hf * FMH + i);
 #pragma unroll
-          for (int j = 0; j < FN; ++j)
+          for (int j = 0; j < SFN; ++j)
             *(vec4*)(stage + i * 16 * RB + w_off + (((2 * j + (wg >> 1)) ^ chunk_xor(wr)) << 4)) = value(hf * FMH + i, j, ctx);
         }
         auto at = [&](int it, int* m, int* n_st) __attribute__((always_inline)) {
           const int r = it * RPI + srow;
           vec8 v = *(const vec8*)(stage + r * RB + schunk * 16);
           if ((r >> 3) & 1) v = vec8{v[4], v[5], v[6], v[7], v[0], v[1], v[2], v[3]};
-          *n_st = col0 + wn * TN + (schunk ^ chunk_xor(r)) * 8;
+          *n_st = col0 + wn * SN + (schunk ^ chunk_xor(r)) * 8;
           *m = row0 + wm * TM + hf * FMH * 16 + r;
           return v;
         };
@@ -1365,12 +1390,12 @@ struct GemmTile {
           for (int it = 0; it < FMH * 16 / RPI; ++it) {
             int m, n_st;
             const vec8 v = at(it, &m, &n_st);
-            if (m < M && n_st + 7 < N) store_16<decltype(kind_tag)::value>(C + (size_t)m * N + n_st, __builtin_bit_cast(i32x4, v));  // (at any element's address)
+            if (m < M && n_st + 7 < N) store_16<decltype(kind_tag)::value>(C + (size_t)m * ld + n_st, __builtin_bit_cast(i32x4, v));  // (at any element's address)
           }
         };
         if (p.c_store == kStoreThrough) store_pass(std::integral_constant<int, kStoreThrough>{});  // (uniform)
         else store_pass(std::integral_constant<int, kStoreCached>{});
-        if ((N & 7) != 0 && col0 + wn * TN + TN > N) {  // the row's last chunk
+        if ((N & 7) != 0 && col0 + wn * SN + SN > N) {  // the row's last chunk
           // (a loop, for its length; unrolled behind a side job, where the loop makes the compiler drain every load in front of the
           // first LDS read of each K tile of the 8-byte units' K loop: 1117 x 6352 x 7616 with 58 Mi elements 144 -> 161 us)
           constexpr int AT_ONCE = SIDE ? FMH * 16 / RPI : 1;
@@ -1381,7 +1406,7 @@ struct GemmTile {
             if (m < M && n_st < N && n_st + 7 >= N) {
 #pragma unroll
               for (int e = 0; e < 7; ++e)
-                if (n_st + e < N) C[(size_t)m * N + n_st + e] = v[e];
+                if (n_st + e < N) C[(size_t)m * ld + n_st + e] = v[e];
             }
           }
         }
@@ -1391,7 +1416,7 @@ struct GemmTile {
     if (EPI == kEpiStore || EPI == kEpiStoreSide) {
       T* C = (T*)p.C;
       __syncthreads();  // every wavefront is done with the last tile, and no fill is still landing
-      staged_store(C, std::integral_constant<int, 0>{}, [](int) { return 0; },
+      staged_store(C, N, std::integral_constant<int, 0>{}, [](int) { return 0; },
                    [&](int i, int j, int) {
                      vec4 v;
 #pragma unroll
@@ -1415,6 +1440,29 @@ struct GemmTile {
           y[done + tid] = silu_16<T>(x[done + tid]);
         }
       }
+    } else if constexpr (GATED) {
+      // Blocks 2 j and 2 j + 1 are the gate and the up factor of the same columns.  The product is taken in fp32 and rounded once;
+      // the factors that a backward pass will need are rounded to the operands' type, as any activation that is kept.
+      __syncthreads();
+      auto factor = [&](int up) {
+        return [&acc, up](int i, int j, int) {
+          vec4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][2 * j + up][e];
+          return v;
+        };
+      };
+      if (p.gu) {  // (uniform; a wavefront's staging area is its own, and its LDS accesses stay in order)
+        staged_store((T*)p.gu, 2 * N, std::integral_constant<int, 0>{}, [](int) { return 0; }, factor(0));
+        staged_store((T*)p.gu + N, 2 * N, std::integral_constant<int, 0>{}, [](int) { return 0; }, factor(1));
+      }
+      staged_store((T*)p.C, N, std::integral_constant<int, 0>{}, [](int) { return 0; },
+                   [&](int i, int j, int) {
+                     vec4 v;
+#pragma unroll
+                     for (int e = 0; e < 4; ++e) v[e] = (T)gated_f32<T>(acc[i][2 * j][e], acc[i][2 * j + 1][e]);
+                     return v;
+                   });
     } else if constexpr (LOOP) {
       // Walk the tiles id, id + grid, ...  After the K loop of one tile every LDS slot is dead: the
       // first operand tiles of the next one go into the slots they belong to (A 0 .. AST-2, B 0 ..
@@ -1563,7 +1611,7 @@ struct GemmTile {
       // 5. normalise the accumulators and store Y (through LDS, behind the row statistics)
       T* Y = (T*)p.C;
       struct RowStat { float mean, rstd; };
-      staged_store(Y, std::integral_constant<int, BM * 2 * 4>{},
+      staged_store(Y, N, std::integral_constant<int, BM * 2 * 4>{},
                    [&](int i) {
                      const int rl = wm * TM + i * 16 + (lane & 15);
                      return RowStat{red[rl * 2 + 0], red[rl * 2 + 1]};

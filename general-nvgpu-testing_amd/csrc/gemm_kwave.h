@@ -50,6 +50,11 @@ struct KwSideParams : KwParams {
   long long side_count;
 };
 
+// Gated layer (gemm_kernel.h: kEpiGated): B is [2 N][K], the 16-column blocks of a tile are gate and up rows in turn.
+struct KwGatedParams : KwParams {
+  void* gu;  // 16-bit [M][2 N], the two factors before the activation; null: not asked for
+};
+
 // GEMM+LayerNorm: the exchange of gemm_kernel.h, workgroups in one of the orders without padding.
 struct KwLnParams : KwParams {
   float* stats;  // 8-byte words [tiles_m][tiles_n][ROWS] = (mean, tag)
@@ -95,7 +100,7 @@ BEAM_HD int kw_kmajor_offset(int k, int n, int cols) {
 }
 
 // AG groups of 8 rows of A, CB blocks of 16 columns, NW wavefronts, S LDS slots of one K tile for each.
-template <typename T, int AG, int CB, int NW, int S, KwRows MODE, bool KMAJOR>
+template <typename T, int AG, int CB, int NW, int S, KwRows MODE, bool KMAJOR, bool GATED = false>
 struct KwTile {
   using Traits = ElemTraits<T>;
   using vec8 = typename Traits::vec8;
@@ -104,6 +109,7 @@ struct KwTile {
   static constexpr int MB = AG < 2 ? 1 : AG / 2;  // blocks of 16 rows
   static constexpr int ROWS = AG * 8;
   static constexpr int COLS = 16 * CB;
+  static constexpr int CN = GATED ? COLS / 2 : COLS;  // columns of C
   static constexpr int NT = NW * 64;
   static constexpr int LB = 2 * CB;
   static constexpr int LOADS = AG + LB;                // buffer loads of 1 KiB per K tile
@@ -117,6 +123,7 @@ struct KwTile {
   static_assert(S >= 1 && (S - 1) * LOADS < 64, "vmcnt range");
   static_assert(LDS_BYTES <= 160 * 1024 && SUM_BYTES <= S * SLOT, "LDS; the sums reuse the ring");
   static_assert(CG == 4 || CG == 8 || CG == 16, "sum layout");
+  static_assert(!GATED || (!KMAJOR && CB % 2 == 0), "pairs of blocks");
 
   // Where the four sums of (row, column group) lie: 16 rows of one column group (what a store of a block writes) and 16
   // neighbouring column groups or rows (what a thread's neighbours read) are 16 different 16-byte slots of a bank sweep.
@@ -126,7 +133,7 @@ struct KwTile {
   static __device__ __forceinline__ void multiply(const KwParams& p, int row0, int col0, int wave, int lane, char* ring, f32x4 (&acc)[MB][CB]) {
     const int M = p.M, N = p.N, K = p.K;
     const int rows_a = M - row0 < ROWS ? M - row0 : ROWS;
-    const int rows_b = N - col0 < COLS ? N - col0 : COLS;
+    const int rows_b = N - col0 < CN ? N - col0 : CN;
     // Whole chunks of 8 elements, and up to 8 that come last.  K-major rows that are not whole chunks: the very last row is
     // always among those, so that every row that is fetched has another one behind it and may be read past its end.
     const bool n_odd = KMAJOR && (N & 7) != 0;
@@ -143,6 +150,8 @@ struct KwTile {
     constexpr int LEAD = SHIFT ? kRowBytes : 0;
     const __amdgpu_buffer_rsrc_t ra = make_rsrc((const char*)a_base - LEAD, (unsigned)rows_a * (unsigned)K * 2u + LEAD);
     const __amdgpu_buffer_rsrc_t rb = make_rsrc((const char*)b_base - LEAD, KMAJOR ? 0u : (unsigned)rows_b * (unsigned)K * 2u + LEAD);
+    const T* const up_base = GATED ? b_base + (size_t)N * K : b_base;  // rows of the odd blocks
+    const __amdgpu_buffer_rsrc_t rup = GATED ? make_rsrc((const char*)up_base - LEAD, (unsigned)rows_b * (unsigned)K * 2u + LEAD) : rb;
     const unsigned row_bytes = (unsigned)K * 2u;
     // chunks between the start of row r's first line and the row (rows 16 apart share it: exact for K % 4 == 0)
     auto phase_of = [&](const T* base, int r) __attribute__((always_inline)) {
@@ -170,6 +179,7 @@ struct KwTile {
     };
     const Lane la0 = lane_of(a_base, 0), la1 = lane_of(a_base, 1);
     const Lane lb0 = lane_of(b_base, 0), lb1 = lane_of(b_base, 1);
+    const Lane lu0 = GATED ? lane_of(up_base, 0) : lb0, lu1 = GATED ? lane_of(up_base, 1) : lb1;
     // K-major B: chunk position q of a slot is row k = q / CPR (after kw_kmajor_row, its own inverse), chunk q % CPR ^ swizzle
     constexpr int CPR = COLS / 8;
     unsigned voff_b[LB];
@@ -204,8 +214,14 @@ struct KwTile {
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)(dst + A_BYTES + i * 1024), 16, (int)voff_b[i], 0, 0, 0);
       } else {
 #pragma unroll
-        for (int i = 0; i < LB; ++i)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(dst + A_BYTES + i * 1024), 16, off_of(i & 1 ? lb1 : lb0, i), 0, 0, 0);
+        for (int i = 0; i < LB; ++i) {
+          if constexpr (GATED) {  // loads 4 j, 4 j + 1 bring gate rows, the next two the up rows of the same columns
+            const int off = off_of(i & 2 ? (i & 1 ? lu1 : lu0) : (i & 1 ? lb1 : lb0), (i >> 2) * 2 + (i & 1));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(i & 2 ? rup : rb, (__attribute__((address_space(3))) void*)(dst + A_BYTES + i * 1024), 16, off, 0, 0, 0);
+          } else {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (__attribute__((address_space(3))) void*)(dst + A_BYTES + i * 1024), 16, off_of(i & 1 ? lb1 : lb0, i), 0, 0, 0);
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < AG; ++i)
@@ -220,13 +236,14 @@ struct KwTile {
 
     // Fragments: lane l reads row l & 15, chunk 4 * kk + (l >> 4) of a block.
     int frag_off[2];
-    bool late_a[2], late_b[2];
+    bool late_a[2], late_b[2], late_up[2];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       const int c = 4 * kk + (lane >> 4);
       frag_off[kk] = lds_offset(lane & 15, c);
       late_a[kk] = SHIFT && c + phase_of(a_base, lane & 15) >= 8;
       late_b[kk] = SHIFT && !KMAJOR && c + phase_of(b_base, lane & 15) >= 8;
+      late_up[kk] = SHIFT && GATED && c + phase_of(up_base, lane & 15) >= 8;
     }
     int bfrag_off[CB];
     if constexpr (KMAJOR) {
@@ -296,7 +313,7 @@ struct KwTile {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-        for (int j = 0; j < CB; ++j) before.b[kk][j] = KMAJOR ? now.b[kk][j] : pick(late_b[kk], now.b[kk][j], before.b[kk][j]);
+        for (int j = 0; j < CB; ++j) before.b[kk][j] = KMAJOR ? now.b[kk][j] : pick(GATED && (j & 1) ? late_up[kk] : late_b[kk], now.b[kk][j], before.b[kk][j]);
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
           before.a[kk][i] = pick(late_a[kk], now.a[kk][i], before.a[kk][i]);
@@ -361,7 +378,7 @@ struct KwTile {
 #pragma unroll
           for (int e = 0; e < 8; ++e) fb[j][e] = lane < 16 && e < rem && nn < N ? ((const T*)p.B)[(size_t)(k8 * 8 + e) * N + nn] : (T)0.0f;
         } else {
-          fb[j] = row_end(b_base, rows_b, j);
+          fb[j] = GATED ? row_end(j & 1 ? up_base : b_base, rows_b, j >> 1) : row_end(b_base, rows_b, j);
         }
       }
 #pragma unroll
@@ -392,9 +409,9 @@ struct KwTile {
     for (int w = 1; w < NW; ++w) v += part[w];
     return v;
   }
-  static __device__ __forceinline__ void store_quad(T* C, int m, int n, int N, vec4 v) {
+  static __device__ __forceinline__ void store_quad(T* row, int n, int N, vec4 v) {
     typedef T at_element __attribute__((ext_vector_type(4), aligned(2)));  // C lies at any element's address
-    T* dst = C + (size_t)m * N + n;
+    T* dst = row + n;
     if (n + 3 < N) {
       *(at_element*)dst = v;
     } else {
@@ -426,7 +443,46 @@ struct KwTile {
       vec4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
-      store_quad((T*)p.C, m, n, p.N, o);
+      store_quad((T*)p.C + (size_t)m * p.N, n, p.N, o);
+    }
+  }
+
+  // Quad (row, column group) of C: the gate's sums lie in the even blocks, the up rows' in the odd ones.
+  static __device__ __forceinline__ void run_gated(const KwGatedParams& p, char* smem) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const TileCoord tc = tile_of_workgroup(blockIdx.x, p.tiles_m, p.tiles_n, p.group_m, p.divs);
+    const int row0 = tc.tm * ROWS, col0 = tc.tn * CN;
+    char* const ring = smem + wave * (S * SLOT);
+    f32x4 acc[MB][CB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    multiply(p, row0, col0, wave, lane, ring, acc);
+    meet(lane, ring, acc);
+    constexpr int HG = CG / 2;  // column groups of C
+#pragma unroll
+    for (int q0 = 0; q0 < QUADS / 2; q0 += NT) {
+      const int q = q0 + (int)threadIdx.x;
+      const int row = q / HG, cg = q % HG;
+      const int m = row0 + row, n = col0 + cg * 4;
+      if (q >= QUADS / 2 || row >= ROWS || m >= p.M || n >= p.N) continue;
+      const int at = row * CG + (cg >> 2) * 8 + (cg & 3);
+      const f32x4 g = total(smem, at), u = total(smem, at + 4);
+      vec4 h, g16, u16;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[e] = (T)gated_f32<T>(g[e], u[e]);
+        g16[e] = (T)g[e];
+        u16[e] = (T)u[e];
+      }
+      store_quad((T*)p.C + (size_t)m * p.N, n, p.N, h);
+      if (p.gu) {
+        T* const row_of_gu = (T*)p.gu + (size_t)m * 2 * p.N;
+        store_quad(row_of_gu, n, p.N, g16);
+        store_quad(row_of_gu + p.N, n, p.N, u16);
+      }
     }
   }
 
@@ -525,7 +581,7 @@ struct KwTile {
       vec4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = (T)((v[u][e] - mean) * rstd * (float)g[e] + (float)b[e]);
-      store_quad((T*)p.C, m, n, N, o);
+      store_quad((T*)p.C + (size_t)m * N, n, N, o);
     }
   }
 };
@@ -551,6 +607,12 @@ __global__ void __launch_bounds__(NW * 64, 2) gemm_kwave_side_kernel(const KwSid
     return;
   }
   KwTile<T, AG, CB, NW, S, MODE, false>::run(p, smem);
+}
+
+template <typename T, int AG, int CB, int NW, int S, KwRows MODE>
+__global__ void __launch_bounds__(NW * 64, 2) gemm_kwave_gated_kernel(const KwGatedParams p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  KwTile<T, AG, CB, NW, S, MODE, false, true>::run_gated(p, smem);
 }
 
 template <typename T, int AG, int CB, int NW, int S, KwRows MODE>

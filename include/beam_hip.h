@@ -260,6 +260,24 @@ int beam_silu(const void* X, void* Y, long long count, int dtype, void* stream);
 int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, int dtype, const beam_tile_cfg* cfg,
                    void* stream);
 
+/* ---- gated layer, forward and backward ------------------------------------------------------ */
+
+/* H[M][N] = silu(G) * U with G = A . B[0..N)^T and U = A . B[N..2N)^T: B is [2N][K], the N rows of the gate's projection in front
+ * of the N rows of the other one; both products, the activation and their product in one launch, from the fp32 sums, rounded
+ * once.  GU, if not null: [M][2N], G and U rounded to the dtype, what the backward pass takes.  Any M, N, K and any element's
+ * address.  H and GU must not overlap each other or an input.  No counterpart in the reference (its SiLU,
+ * cuda/cute_kernels/cute_gemm_ln.cu:191-192, is a job beside a product). */
+int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, void* stream);
+
+/* The gradients of that layer: with s = 1 / (1 + exp(-G)), D = [dH * U * s * (1 + G * (1 - s)), dH * G * s] ([M][2N], rounded to
+ * the dtype for the products that follow), dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or
+ * dB may be null: not asked for.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches; the workspace (256-byte
+ * aligned, any contents) holds D and its transpose and belongs to the call until it has run: calls that overlap in time need one
+ * each, and so does a captured graph that may run beside another. */
+size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int want_dA, int want_dB);
+int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
+                               int dtype, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- timing ------------------------------------------------------------------------------- */
 
 /* Which operation beam_bench times. */
