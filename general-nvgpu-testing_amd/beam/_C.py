@@ -108,6 +108,14 @@ def _load() -> ctypes.CDLL:
     L.beam_gemmrc_gated_backward_workspace_bytes.argtypes = [i, i, i, i]
     L.beam_gemmrc_gated_backward_workspace_bytes.restype = sz
     L.beam_gemmrc_gated_backward.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
+    L.beam_mxfp4_scale_bytes.argtypes = [i, i]
+    L.beam_mxfp4_scale_bytes.restype = sz
+    L.beam_mxfp4_quantize.argtypes = [vp, vp, vp, i, i, i, vp]
+    L.beam_mxfp4_dequantize.argtypes = [vp, vp, vp, i, i, i, vp]
+    L.beam_gemmrc_mxfp4.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp]
+    L.beam_linear_mxfp4_workspace_bytes.argtypes = [i, i]
+    L.beam_linear_mxfp4_workspace_bytes.restype = sz
+    L.beam_linear_mxfp4.argtypes = [vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
     L.beam_bench.argtypes = [i, ctypes.POINTER(_Problem), cfgp, i, i, vp, ctypes.POINTER(ctypes.c_float)]
     L.beam_stream_create.argtypes = [ctypes.POINTER(vp)]
     L.beam_stream_destroy.argtypes = [vp]
@@ -134,6 +142,7 @@ def _load() -> ctypes.CDLL:
     L.beam_dbg_ln_plan_bytes.restype = sz
     L.beam_dbg_assume_compute_units.argtypes = [i]
     L.beam_dbg_small_tile.argtypes = [i, i, i, i, i] + [ctypes.POINTER(i)] * 4
+    L.beam_dbg_mx_tile.argtypes = [i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_gated_tile.argtypes = [i, i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_nn_off_lines_tile.argtypes = [i, i, i, cfgp, cfgp, ctypes.POINTER(i)]
     L.beam_dbg_off_lines_tile.argtypes = L.beam_dbg_ln_line_tile.argtypes = [i, i, i, cfgp, ctypes.POINTER(i)]
@@ -650,6 +659,97 @@ def gemmrc_gated_backward(dh, gu, a, b, da=None, db=None) -> None:
         need = lib.beam_gemmrc_gated_backward_workspace_bytes(M, N2 // 2, da is not None, db is not None)
         ws, keep = _call_workspace(a, need)
         _check(lib.beam_gemmrc_gated_backward(pdh, pgu, pa, pb, pda, pdb, M, N2 // 2, K, d, ws, need, _stream_of(a)))
+        del keep
+
+
+# ---------------------------------------------------------------------------- MXFP4
+
+
+def _describe_bytes(x, name: str, shape):
+    """Pointer of an array of single bytes (torch: uint8, or the 4-bit and scale types of that size) of the given shape."""
+    if _Tensor is not None and isinstance(x, _Tensor):
+        if not x.is_cuda:
+            raise BeamError(1, "tensor is not on the GPU")
+        if not x.is_contiguous():
+            raise BeamError(1, "tensor is not contiguous")
+        if x.dtype not in _BYTE_TYPES:
+            raise BeamError(2, f"{name} must be uint8, not {x.dtype}")
+        p, s = x.data_ptr(), x.shape
+    elif isinstance(x, DeviceArray):
+        if x.itemsize != 1:
+            raise BeamError(2, f"{name} must have elements of one byte")
+        p, s = x.ptr, x.shape
+    else:
+        return _describe(x)[0]  # words the error
+    if tuple(s) != shape:
+        raise BeamError(1, f"{name} has shape {tuple(s)}, expected {shape}")
+    return p
+
+
+_BYTE_TYPES = () if _torch is None else tuple(
+    getattr(_torch, t) for t in ("uint8", "float4_e2m1fn_x2", "float8_e8m0fnu") if hasattr(_torch, t))
+
+
+def _held(x, scales, name: str, rows: int, K: int):
+    if K % 32:
+        raise BeamError(1, f"{name} has {K} columns, not a whole number of blocks of 32")
+    return (_describe_bytes(x, name, (rows, K // 2)),
+            _describe_bytes(scales, f"{name}'s scales", mxfp4_scales_shape(rows, K)))
+
+
+def _rows_held(x, name: str):
+    """(rows, columns) of elements in MXFP4."""
+    s = getattr(x, "shape", ())
+    if len(s) != 2:
+        raise BeamError(1, f"{name} must be 2-D")
+    if max(s) > 0x3FFFFFFF:
+        raise BeamError(2, f"{name} has shape {tuple(s)}: too large")
+    return s[0], 2 * s[1]
+
+
+def mxfp4_scales_shape(rows: int, K: int):
+    """Shape of the scales (uint8) of [rows, K] in MXFP4: the one of row r, columns 32 b .. 32 b + 31 is [b // 8, r, b % 8]."""
+    return ((K + 255) // 256, rows, 8)
+
+
+def mxfp4_quantize(x, q, scales) -> None:
+    """x [M, K], 16-bit, in MXFP4: q [M, K / 2] bytes of two elements each (the even column in the low half), scales
+    mxfp4_scales_shape(M, K).  K is a multiple of 32."""
+    with _same_device(x, q, scales):
+        px, M, K, d = _matrix(x, "x")
+        pq, ps = _held(q, scales, "q", M, K)
+        _check(lib.beam_mxfp4_quantize(px, pq, ps, M, K, d, _stream_of(x)))
+
+
+def mxfp4_dequantize(q, scales, x) -> None:
+    """x [M, K], 16-bit: the values that q and scales hold."""
+    with _same_device(x, q, scales):
+        px, M, K, d = _matrix(x, "x")
+        pq, ps = _held(q, scales, "q", M, K)
+        _check(lib.beam_mxfp4_dequantize(pq, ps, px, M, K, d, _stream_of(x)))
+
+
+def gemmrc_mxfp4(a, a_scales, b, b_scales, c) -> None:
+    """c = a @ b.T of two operands in MXFP4 (mxfp4_quantize): a stands for [M, K], b for [N, K]; c [M, N] is 16-bit."""
+    with _same_device(a, a_scales, b, b_scales, c):
+        M, K = _rows_held(a, "a")
+        N = _rows_held(b, "b")[0]
+        pa, psa = _held(a, a_scales, "a", M, K)
+        pb, psb = _held(b, b_scales, "b", N, K)
+        pc, _, _, d = _matrix(c, "c", M, N)
+        _check(lib.beam_gemmrc_mxfp4(pa, psa, pb, psb, pc, M, N, K, d, _stream_of(c)))
+
+
+def linear_mxfp4(a, b, b_scales, c) -> None:
+    """c = a @ b.T with a [M, K] in 16 bits, quantised to MXFP4 in the call, and b in MXFP4 (standing for [N, K])."""
+    with _same_device(a, b, b_scales, c):
+        pa, M, K, d = _matrix(a, "a")
+        N = _rows_held(b, "b")[0]
+        pb, psb = _held(b, b_scales, "b", N, K)
+        pc = _matrix(c, "c", M, N, d)[0]
+        need = lib.beam_linear_mxfp4_workspace_bytes(M, K)
+        ws, keep = _call_workspace(a, need)
+        _check(lib.beam_linear_mxfp4(pa, pb, psb, pc, M, N, K, d, ws, need, _stream_of(a)))
         del keep
 
 

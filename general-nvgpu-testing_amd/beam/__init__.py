@@ -20,12 +20,17 @@ from ._C import (  # noqa: F401
     gemmrc_gated,
     gemmrc_gated_backward,
     gemmrc_ln,
+    gemmrc_mxfp4,
     gemmrc_spec,
     gemmrc_splitk,
     gemmrc_splitk_spec,
     list_configs,
     library_path,
+    linear_mxfp4,
     matmul,
+    mxfp4_dequantize,
+    mxfp4_quantize,
+    mxfp4_scales_shape,
     parallel_gemmrc_silu,
     silu,
 )

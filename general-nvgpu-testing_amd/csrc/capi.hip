@@ -19,6 +19,7 @@
 #include "../../include/beam_hip_debug.h"
 #include "aux_kernels.h"
 #include "gated.h"
+#include "mx.h"
 #include "kernel_set.h"
 #include "tile_map.h"
 
@@ -1108,6 +1109,144 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
   return BEAM_OK;
 }
 
+// ---- MXFP4 ------------------------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+// Columns of an MXFP4 operand: a tile's descriptor, 256 rows of K / 2 bytes, and any offset past it fit 32 bits.
+constexpr int kMxMaxK = 1 << 22;
+
+int check_mx(int rows, int K, int dtype) {
+  if (rows < 0 || K < 0) return fail(BEAM_ERR_INVALID, "negative dimension (%d rows, K=%d)", rows, K);
+  if (K % 32 != 0) return fail(BEAM_ERR_INVALID, "K=%d is not a whole number of blocks of 32", K);
+  if (K > kMxMaxK) return fail(BEAM_ERR_UNSUPPORTED, "K=%d beyond %d", K, kMxMaxK);
+  if (dtype != BEAM_F16 && dtype != BEAM_BF16) return fail(BEAM_ERR_UNSUPPORTED, "dtype %d: only fp16 (0) and bf16 (1)", dtype);
+  return BEAM_OK;
+}
+
+int check_mx_held(const void* elements, const void* scales, const char* what) {
+  if (!elements || !scales) return fail(BEAM_ERR_INVALID, "null pointer to %s", what);
+  if (((uintptr_t)elements & 15) != 0 || ((uintptr_t)scales & 7) != 0) return fail(BEAM_ERR_INVALID, "elements of %s must start on 16 bytes and scales on 8", what);
+  return BEAM_OK;
+}
+
+int check_mx_product(const void* C, int M, int N, int K, int dtype) {
+  int rc;
+  if ((rc = check_mx(M, K, dtype)) || (rc = check_mx(N, K, dtype))) return rc;
+  if (M == 0 || N == 0) return BEAM_OK;
+  if (!C) return fail(BEAM_ERR_INVALID, "null output pointer");
+  if ((uintptr_t)C & 1) return fail(BEAM_ERR_INVALID, "C must be aligned to its 16-bit elements");
+  if ((size_t)M * (size_t)N >= ((size_t)1 << 40) || (size_t)((M + 15) / 16) * (size_t)((N + 15) / 16) > INT32_MAX)
+    return fail(BEAM_ERR_UNSUPPORTED, "M=%d x N=%d too large", M, N);
+  return BEAM_OK;
+}
+
+// What an MXFP4 product runs on: rows x cols, the tile of gemm_mx.h's two kernels.
+struct MxPlan {
+  int rows, cols;
+  bool kwave;
+};
+MxPlan mx_plan(int M, int N, int cus) {
+  static const struct { int rows, cols; } kSmall[] = {{16, 16}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
+  auto tiles = [&](int r, int c) { return ((long)M + r - 1) / r * (((long)N + c - 1) / c); };
+  for (const auto& t : kSmall) {
+    const bool few = M <= 16 && t.rows == 16 && t.cols == 64;
+    if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, true};
+  }
+  if (tiles(256, 256) >= cus) return MxPlan{256, 256, false};
+  if (tiles(256, 128) >= cus) return MxPlan{256, 128, false};
+  if (tiles(128, 128) >= cus) return MxPlan{128, 128, false};
+  return MxPlan{64, 64, false};
+}
+
+int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* sB, void* C, int M, int N, int K, int dtype, hipStream_t st) {
+  const MxPlan plan = mx_plan(M, N, g_dev.cus > 0 ? g_dev.cus : 256);
+  MxParams p;
+  p.A = A;
+  p.B = B;
+  p.sa = (const uint8_t*)sA;
+  p.sb = (const uint8_t*)sB;
+  p.C = C;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.tiles_m = (M + plan.rows - 1) / plan.rows;
+  p.tiles_n = (N + plan.cols - 1) / plan.cols;
+  p.group_m = plan.kwave ? 8 : default_group_m(plan.rows, plan.cols);
+  p.divs = make_tile_divs(p.tiles_m, p.tiles_n, p.group_m);
+  if (plan.kwave) BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx_kwave<_Float16>(plan.rows, plan.cols, a16, p, st) : launch_gemm_mx_kwave<__bf16>(plan.rows, plan.cols, a16, p, st));
+  else BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx<_Float16>(plan.rows, plan.cols, p, st) : launch_gemm_mx<__bf16>(plan.rows, plan.cols, p, st));
+  return BEAM_OK;
+}
+
+// Whether the product quantises its 16-bit operand by itself (gemm_mx.h: A16).
+bool mx_takes_16_bits(int M, int K) { return M <= 16 && K <= kMxKeptColumns; }
+
+}  // namespace
+
+extern "C" {
+
+size_t beam_mxfp4_scale_bytes(int rows, int K) { return rows <= 0 || K <= 0 ? 0 : ((size_t)K + kMxTile - 1) / kMxTile * (size_t)rows * kMxBlocks; }
+
+int beam_mxfp4_quantize(const void* X, void* elements, void* scales, int rows, int K, int dtype, void* stream) {
+  int rc = check_mx(rows, K, dtype);
+  if (rc || rows == 0 || K == 0) return rc;
+  if (!X) return fail(BEAM_ERR_INVALID, "null input pointer");
+  if ((uintptr_t)X & 1) return fail(BEAM_ERR_INVALID, "X must be aligned to its 16-bit elements");
+  if ((rc = check_mx_held(elements, scales, "the result")) || (rc = beam_init())) return rc;
+  BEAM_HIP(launch_mx_quantize(X, (uint8_t*)elements, (uint8_t*)scales, rows, K, dtype, (hipStream_t)stream));
+  return BEAM_OK;
+}
+
+int beam_mxfp4_dequantize(const void* elements, const void* scales, void* X, int rows, int K, int dtype, void* stream) {
+  int rc = check_mx(rows, K, dtype);
+  if (rc || rows == 0 || K == 0) return rc;
+  if (!X) return fail(BEAM_ERR_INVALID, "null output pointer");
+  if ((uintptr_t)X & 1) return fail(BEAM_ERR_INVALID, "X must be aligned to its 16-bit elements");
+  if ((rc = check_mx_held(elements, scales, "the operand")) || (rc = beam_init())) return rc;
+  BEAM_HIP(launch_mx_dequantize((const uint8_t*)elements, (const uint8_t*)scales, X, rows, K, dtype, (hipStream_t)stream));
+  return BEAM_OK;
+}
+
+int beam_gemmrc_mxfp4(const void* A, const void* A_scales, const void* B, const void* B_scales, void* C, int M, int N, int K, int dtype,
+                      void* stream) {
+  int rc = check_mx_product(C, M, N, K, dtype);
+  if (rc || M == 0 || N == 0) return rc;
+  if (K > 0 && ((rc = check_mx_held(A, A_scales, "A")) || (rc = check_mx_held(B, B_scales, "B")))) return rc;
+  if ((rc = beam_init())) return rc;
+  if (K == 0) {
+    BEAM_HIP(launch_zero_u16(C, (size_t)M * N, (hipStream_t)stream));
+    return BEAM_OK;
+  }
+  return run_mx(A, A_scales, false, B, B_scales, C, M, N, K, dtype, (hipStream_t)stream);
+}
+
+size_t beam_linear_mxfp4_workspace_bytes(int M, int K) {
+  if (M <= 0 || K <= 0 || mx_takes_16_bits(M, K)) return 0;
+  return align_up((size_t)M * (size_t)(K / 2), 256) + align_up(beam_mxfp4_scale_bytes(M, K), 256);
+}
+
+int beam_linear_mxfp4(const void* A, const void* B, const void* B_scales, void* C, int M, int N, int K, int dtype, void* ws,
+                      size_t ws_bytes, void* stream) {
+  int rc = check_mx_product(C, M, N, K, dtype);
+  if (rc || M == 0 || N == 0) return rc;
+  if (K == 0) return beam_gemmrc_mxfp4(nullptr, nullptr, nullptr, nullptr, C, M, N, 0, dtype, stream);
+  if (!A) return fail(BEAM_ERR_INVALID, "null input pointer");
+  if ((uintptr_t)A & 1) return fail(BEAM_ERR_INVALID, "A must be aligned to its 16-bit elements");
+  if ((rc = check_mx_held(B, B_scales, "B"))) return rc;
+  const size_t need = beam_linear_mxfp4_workspace_bytes(M, K);
+  if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255) != 0))
+    return fail(BEAM_ERR_WORKSPACE, "workspace of %zu bytes on 256 needed, %zu given", need, ws ? ws_bytes : (size_t)0);
+  if ((rc = beam_init())) return rc;
+  if (need == 0) return run_mx(A, nullptr, true, B, B_scales, C, M, N, K, dtype, (hipStream_t)stream);
+  char* const elements = (char*)ws;
+  char* const scales = elements + align_up((size_t)M * (size_t)(K / 2), 256);
+  BEAM_HIP(launch_mx_quantize(A, (uint8_t*)elements, (uint8_t*)scales, M, K, dtype, (hipStream_t)stream));
+  return run_mx(elements, scales, false, B, B_scales, C, M, N, K, dtype, (hipStream_t)stream);
+}
+
 int beam_silu(const void* X, void* Y, long long count, int dtype, void* stream) {
   if (count < 0) return fail(BEAM_ERR_INVALID, "negative element count %lld", count);
   if (dtype != BEAM_F16 && dtype != BEAM_BF16) return fail(BEAM_ERR_UNSUPPORTED, "dtype %d: only fp16 (0) and bf16 (1)", dtype);
@@ -1905,6 +2044,13 @@ int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, 
   *cols = kw.cols;
   *waves = kw.waves;
   *whole_lines = kw.shift ? 1 : 0;
+  return BEAM_OK;
+}
+
+int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave) {
+  if (!rows || !cols || !kwave || M < 1 || N < 1 || K < 32) return fail(BEAM_ERR_INVALID, "arguments");
+  const MxPlan plan = mx_plan(M, N, g_dev.cus > 0 ? g_dev.cus : 256);
+  *rows = plan.rows, *cols = plan.cols, *kwave = plan.kwave;
   return BEAM_OK;
 }
 

@@ -278,6 +278,32 @@ size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int want_dA, int
 int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
                                int dtype, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- MXFP4: 4-bit elements with a scale for every 32 of them ------------------------------------ */
+
+/* The format (OCP microscaling, MXFP4).  Elements: two to a byte, the even column in the low half, e2m1 (sign, then the code of
+ * 0, 0.5, 1, 1.5, 2, 3, 4, 6): [rows][K / 2] bytes, 16-byte aligned.  Scales: a biased power of two (e8m0: 2^(byte - 127), 255 is NaN)
+ * for every 32 columns of a row: the one of row r, block b is byte [b / 8][r][b % 8] of [ceil(K / 256)][rows][8], 8-byte aligned;
+ * bytes behind a row's last block are written as zeros and never looked at.  K is a multiple of 32, at most 2^22.
+ * (From scales as [rows][K / 32]: pad the columns to a multiple of 8, view as [rows][K / 256][8], exchange the first two axes.)
+ * No counterpart in the reference, whose operands are fp16. */
+size_t beam_mxfp4_scale_bytes(int rows, int K);
+/* X [rows][K] (16-bit, any element's address) in that format: a block's power of two is the one at or below its largest magnitude,
+ * over 4 (at least 2^-127); an element is the nearest value of the eight, ties to the even code, 6 beyond 6.  A block with an infinity or a NaN
+ * in it gets the scale NaN, and is NaN in whatever is made of it. */
+int beam_mxfp4_quantize(const void* X, void* elements, void* scales, int rows, int K, int dtype, void* stream);
+/* The values held, in dtype (rounded to nearest where it cannot hold them). */
+int beam_mxfp4_dequantize(const void* elements, const void* scales, void* X, int rows, int K, int dtype, void* stream);
+/* C[M][N] = A . B^T of two such operands on the scaled matrix instructions, fp32 accumulation, rounded once to dtype.  C at any
+ * element's address. */
+int beam_gemmrc_mxfp4(const void* A, const void* A_scales, const void* B, const void* B_scales, void* C, int M, int N, int K, int dtype,
+                      void* stream);
+/* The same with A [M][K] in 16 bits (dtype, any element's address), quantised in the call: up to 16 rows by the product's own launch,
+ * without workspace; beyond by a launch in front of it, into the workspace (256-byte aligned, any contents; it belongs to the
+ * call until it has run). */
+size_t beam_linear_mxfp4_workspace_bytes(int M, int K);
+int beam_linear_mxfp4(const void* A, const void* B, const void* B_scales, void* C, int M, int N, int K, int dtype, void* ws,
+                      size_t ws_bytes, void* stream);
+
 /* ---- timing ------------------------------------------------------------------------------- */
 
 /* Which operation beam_bench times. */
