@@ -635,6 +635,8 @@ def _matrix(x, name: str, rows: Optional[int] = None, cols: Optional[int] = None
 def gemmrc_gated(a, b, h, gu=None) -> None:
     """h = silu(a @ b[:N].T) * (a @ b[N:].T) in one launch: a [M, K], b [2 N, K] (the gate's rows, then the other projection's),
     h [M, N].  gu [M, 2 N], if given, gets the two factors before the activation, what gemmrc_gated_backward takes."""
+    if _native is not None and (status := _native.gemmrc_gated(a, b, h, gu)) >= 0:
+        return _check(status)
     with _same_device(a, b, h, gu):
         pa, M, K, d = _matrix(a, "a")
         pb, N2, _, _ = _matrix(b, "b", None, K, d)
@@ -648,6 +650,8 @@ def gemmrc_gated(a, b, h, gu=None) -> None:
 def gemmrc_gated_backward(dh, gu, a, b, da=None, db=None) -> None:
     """The gradients of gemmrc_gated: dh [M, N] is h's, gu [M, 2 N] what the forward call wrote; da [M, K] and db [2 N, K] are
     written, either may be left out."""
+    if _native is not None and (status := _native.gemmrc_gated_backward(dh, gu, a, b, da, db)) >= 0:
+        return _check(status)
     with _same_device(dh, gu, a, b, da, db):
         pa, M, K, d = _matrix(a, "a")
         pb, N2, _, _ = _matrix(b, "b", None, K, d)
@@ -715,6 +719,8 @@ def mxfp4_scales_shape(rows: int, K: int):
 def mxfp4_quantize(x, q, scales) -> None:
     """x [M, K], 16-bit, in MXFP4: q [M, K / 2] bytes of two elements each (the even column in the low half), scales
     mxfp4_scales_shape(M, K).  K is a multiple of 32."""
+    if _native is not None and (status := _native.mxfp4_quantize(x, q, scales)) >= 0:
+        return _check(status)
     with _same_device(x, q, scales):
         px, M, K, d = _matrix(x, "x")
         pq, ps = _held(q, scales, "q", M, K)
@@ -723,6 +729,8 @@ def mxfp4_quantize(x, q, scales) -> None:
 
 def mxfp4_dequantize(q, scales, x) -> None:
     """x [M, K], 16-bit: the values that q and scales hold."""
+    if _native is not None and (status := _native.mxfp4_dequantize(q, scales, x)) >= 0:
+        return _check(status)
     with _same_device(x, q, scales):
         px, M, K, d = _matrix(x, "x")
         pq, ps = _held(q, scales, "q", M, K)
@@ -731,6 +739,8 @@ def mxfp4_dequantize(q, scales, x) -> None:
 
 def gemmrc_mxfp4(a, a_scales, b, b_scales, c) -> None:
     """c = a @ b.T of two operands in MXFP4 (mxfp4_quantize): a stands for [M, K], b for [N, K]; c [M, N] is 16-bit."""
+    if _native is not None and (status := _native.gemmrc_mxfp4(a, a_scales, b, b_scales, c)) >= 0:
+        return _check(status)
     with _same_device(a, a_scales, b, b_scales, c):
         M, K = _rows_held(a, "a")
         N = _rows_held(b, "b")[0]
@@ -742,6 +752,8 @@ def gemmrc_mxfp4(a, a_scales, b, b_scales, c) -> None:
 
 def linear_mxfp4(a, b, b_scales, c) -> None:
     """c = a @ b.T with a [M, K] in 16 bits, quantised to MXFP4 in the call, and b in MXFP4 (standing for [N, K])."""
+    if _native is not None and (status := _native.linear_mxfp4(a, b, b_scales, c)) >= 0:
+        return _check(status)
     with _same_device(a, b, b_scales, c):
         pa, M, K, d = _matrix(a, "a")
         N = _rows_held(b, "b")[0]

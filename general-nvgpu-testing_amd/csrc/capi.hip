@@ -287,6 +287,7 @@ GemmParams base_params(const void* A, const void* B, int M, int N, int K, const 
   p.K = K;
   p.tiles_m = (M + c.block_m - 1) / c.block_m;
   p.tiles_n = (N + c.block_n - 1) / c.block_n;
+  p.b_rows = K;
   p.k_slice = ((K + kBK - 1) / kBK) * kBK;
   if (p.k_slice == 0) p.k_slice = kBK;
   p.splits = 1;
@@ -798,15 +799,17 @@ void kw_params(KwParams* p, const KwPlan& plan, const void* A, const void* B, vo
   p->M = M;
   p->N = N;
   p->K = K;
+  p->b_rows = K;
   p->tiles_m = (M + plan.rows - 1) / plan.rows;
   p->tiles_n = (N + plan.cols - 1) / plan.cols;
   p->group_m = 8;
   p->divs = make_tile_divs(p->tiles_m, p->tiles_n, p->group_m);
 }
 
-hipError_t run_kwave(const KwPlan& plan, const void* A, const void* B, void* C, int M, int N, int K, int dtype, bool b_kmajor, hipStream_t st) {
+hipError_t run_kwave(const KwPlan& plan, const void* A, const void* B, void* C, int M, int N, int K, int dtype, bool b_kmajor, hipStream_t st, int b_rows = -1) {
   KwParams p;
   kw_params(&p, plan, A, B, C, M, N, K);
+  if (b_rows >= 0) p.b_rows = b_rows;
   return dtype == BEAM_F16 ? launch_gemm_kwave<_Float16>(plan, p, b_kmajor, st) : launch_gemm_kwave<__bf16>(plan, p, b_kmajor, st);
 }
 
@@ -906,8 +909,12 @@ int beam_gemmrc(const void* A, const void* B, void* C, int M, int N, int K, int 
   return BEAM_OK;
 }
 
-int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, int dtype, const beam_tile_cfg* cfg,
-                   void* stream) {
+}  // extern "C"
+
+namespace {
+
+// beam_matmul_nn for a B of b_rows rows, K or, with zeros in A's columns behind them, up to 63 fewer (GemmParams::b_rows).
+int matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, int b_rows, int dtype, const beam_tile_cfg* cfg, void* stream) {
   bool generic;
   int rc = check_problem(A, B, C, M, N, K, dtype, &generic);
   if (rc) return rc;
@@ -925,7 +932,7 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
   }
   if (!cfg) {
     if (const KwPlan kw = kw_plan(M, N, K, true, false, true, row_starts(A, B, K, true), g_dev.cus > 0 ? g_dev.cus : 256); kw.rows) {
-      BEAM_HIP(run_kwave(kw, A, B, C, M, N, K, dtype, true, st));
+      BEAM_HIP(run_kwave(kw, A, B, C, M, N, K, dtype, true, st, b_rows));
       return BEAM_OK;
     }
   }
@@ -981,6 +988,7 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
   }
   GemmParams p = base_params(A, B, M, N, K, c);
   p.C = C;
+  p.b_rows = b_rows;
   const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
   if (w4_fits && w4_named) {
     const long tiles = (long)p.tiles_m * p.tiles_n;
@@ -992,6 +1000,15 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
   GemmLauncher one_group = cfg ? nullptr : deep_one_group(*ks, c, M, N, K, dtype, true, cus);
   BEAM_HIP((one_group ? one_group : ks->launch_kmajor[dtype][c.pipeline])(p, dim3((unsigned)(p.tiles_m * p.tiles_n), 1, 1), st));
   return BEAM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, int dtype, const beam_tile_cfg* cfg,
+                   void* stream) {
+  return matmul_nn(A, B, C, M, N, K, K, dtype, cfg, stream);
 }
 
 // ---- gated layer ------------------------------------------------------------------------------
@@ -1080,10 +1097,14 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
   return BEAM_OK;
 }
 
+// Columns of the backward pass' D and of its transpose: whole lines (gated_line), so that the products read rows on lines whatever
+// N and M are, where these can run with fewer rows of B than that (matmul_nn); the workspace always has room for them.
+// us, rows as long as they are -> whole lines: 1001 x 2001 x 2000 bf16, dA 31.3 -> GATED_DA, dB 27.0 -> GATED_DB.
+static int gated_line(int n) { return (n + kBK - 1) / kBK * kBK; }
+
 size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int want_dA, int want_dB) {
-  if (M <= 0 || N <= 0) return 0;
-  const size_t one = align_up((size_t)M * 2 * N * 2, 256);
-  return (want_dA ? one : 0) + (want_dB ? one : 0);
+  if (M <= 0 || N <= 0 || N > INT32_MAX / 4) return 0;
+  return (want_dA ? align_up((size_t)M * gated_line(2 * N) * 2, 256) : 0) + (want_dB ? align_up((size_t)2 * N * gated_line(M) * 2, 256) : 0);
 }
 
 int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
@@ -1102,10 +1123,12 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
     return fail(BEAM_ERR_WORKSPACE, "workspace of %zu bytes on 256 needed, %zu given", need, ws ? ws_bytes : (size_t)0);
   if ((rc = beam_init())) return rc;
   char* const d = (char*)ws;
-  char* const dt = d + (dA ? align_up((size_t)M * 2 * N * 2, 256) : 0);
-  if (M > 0 && N > 0) BEAM_HIP(launch_gated_gradients(dH, GU, dA ? d : nullptr, dB ? dt : nullptr, M, N, dtype, (hipStream_t)stream));
-  if (dA && (rc = beam_matmul_nn(d, B, dA, M, K, 2 * N, dtype, nullptr, stream))) return rc;
-  if (dB && (rc = beam_matmul_nn(dt, A, dB, 2 * N, K, M, dtype, nullptr, stream))) return rc;
+  char* const dt = d + (dA ? align_up((size_t)M * gated_line(2 * N) * 2, 256) : 0);
+  const bool lines = K % 8 == 0 && K <= (1 << 23) && gated_line(2 * N) <= kMaxK && gated_line(M) <= kMaxK;
+  const int cols_d = lines ? gated_line(2 * N) : 2 * N, cols_dt = lines ? gated_line(M) : M;
+  if (M > 0 && N > 0) BEAM_HIP(launch_gated_gradients(dH, GU, dA ? d : nullptr, dB ? dt : nullptr, M, N, cols_d, cols_dt, dtype, (hipStream_t)stream));
+  if (dA && (rc = matmul_nn(d, B, dA, M, K, cols_d, 2 * N, dtype, nullptr, stream))) return rc;
+  if (dB && (rc = matmul_nn(dt, A, dB, 2 * N, K, cols_dt, M, dtype, nullptr, stream))) return rc;
   return BEAM_OK;
 }
 

@@ -58,7 +58,9 @@ template <> hipError_t launch_gated_kwave<__bf16>(const KwPlan&, const KwGatedPa
 // Any sizes, element by element (what the tiled kernels refuse: K below 8 or beyond a descriptor).
 hipError_t launch_gated_plain(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, hipStream_t stream);
 
-// D [M][2 N] and DT [2 N][M] (either may be null): the gradients of gate and up factor from dH [M][N] and GU [M][2 N].
-hipError_t launch_gated_gradients(const void* dH, const void* GU, void* D, void* DT, int M, int N, int dtype, hipStream_t stream);
+// D [M][cols_d] and DT [2 N][cols_dt] (either may be null): the gradients of gate and up factor from dH [M][N] and GU [M][2 N],
+// their 2 N and M columns followed by up to 63 zeros.
+hipError_t launch_gated_gradients(const void* dH, const void* GU, void* D, void* DT, int M, int N, int cols_d, int cols_dt, int dtype,
+                                  hipStream_t stream);
 
 }  // namespace beam

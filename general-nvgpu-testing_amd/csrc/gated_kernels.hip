@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256) gated_plain_kernel(const T* __restrict__ 
 // column's number over 8, so that the 8 threads of a row write to different banks; DT then leaves in 128-byte runs.
 template <typename T>
 __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restrict__ dH, const T* __restrict__ GU, T* __restrict__ D,
-                                                              T* __restrict__ DT, int M, int N, int tiles_n) {
+                                                              T* __restrict__ DT, int M, int N, int cols_d, int cols_dt, int tiles_n) {
   typedef T vec8 __attribute__((ext_vector_type(8)));
   typedef T vec8_at_element __attribute__((ext_vector_type(8), aligned(2)));  // rows start at any element
   typedef T pair_t __attribute__((ext_vector_type(2)));
@@ -75,17 +75,25 @@ __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restric
       du[h][e] = (T)(df * (gf * s));
     }
     if (D && m < M) {
+      T* const row = D + (size_t)m * cols_d + n;
       if (n + 7 < N) {
-        *(vec8_at_element*)(D + at_g) = dg[h];
-        *(vec8_at_element*)(D + at_g + N) = du[h];
+        *(vec8_at_element*)row = dg[h];
+        *(vec8_at_element*)(row + N) = du[h];
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (n + e < N) {
-            D[at_g + e] = dg[h][e];
-            D[at_g + N + e] = du[h][e];
+            row[e] = dg[h][e];
+            row[N + e] = du[h][e];
           }
       }
+    }
+  }
+  if (D && tn == tiles_n - 1) {  // (uniform) the zeros behind its rows
+    const int more = cols_d - 2 * N;
+    for (int i = threadIdx.x; i < R * more; i += 256) {
+      const int row = i / more, m = m0 + row;
+      if (m < M) D[(size_t)m * cols_d + 2 * N + (i - row * more)] = (T)0.0f;
     }
   }
   if (!DT) return;  // (uniform)
@@ -102,15 +110,15 @@ __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restric
     const int q = it * 256 + (int)threadIdx.x;
     const int chunk = q & 7, col = (q >> 3) & (C - 1), up = q >> 9;
     const int m = m0 + 8 * chunk;
-    if (n0 + col >= N || m >= M) continue;
+    if (n0 + col >= N || m >= cols_dt) continue;
     const vec8 v = *(const vec8*)(turned + up * C * R + col * R + ((chunk ^ (col >> 3)) << 3));
-    T* const out = DT + ((size_t)up * N + n0 + col) * M + m;
-    if (m + 7 < M) {
+    T* const out = DT + ((size_t)up * N + n0 + col) * cols_dt + m;
+    if (m + 7 < cols_dt) {  // (behind M these are zeros)
       *(vec8_at_element*)out = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (m + e < M) out[e] = v[e];
+        if (m + e < cols_dt) out[e] = v[e];
     }
   }
 }
@@ -127,13 +135,14 @@ hipError_t launch_gated_plain(const void* A, const void* B, void* H, void* GU, i
   return hipGetLastError();
 }
 
-hipError_t launch_gated_gradients(const void* dH, const void* GU, void* D, void* DT, int M, int N, int dtype, hipStream_t stream) {
+hipError_t launch_gated_gradients(const void* dH, const void* GU, void* D, void* DT, int M, int N, int cols_d, int cols_dt, int dtype,
+                                  hipStream_t stream) {
   const int tiles_n = (N + 63) / 64;
   const dim3 grid((unsigned)((size_t)((M + 63) / 64) * tiles_n));
   if (dtype == BEAM_BF16)
-    hipLaunchKernelGGL(gated_gradients_kernel<__bf16>, grid, dim3(256), 0, stream, (const __bf16*)dH, (const __bf16*)GU, (__bf16*)D, (__bf16*)DT, M, N, tiles_n);
+    hipLaunchKernelGGL(gated_gradients_kernel<__bf16>, grid, dim3(256), 0, stream, (const __bf16*)dH, (const __bf16*)GU, (__bf16*)D, (__bf16*)DT, M, N, cols_d, cols_dt, tiles_n);
   else
-    hipLaunchKernelGGL(gated_gradients_kernel<_Float16>, grid, dim3(256), 0, stream, (const _Float16*)dH, (const _Float16*)GU, (_Float16*)D, (_Float16*)DT, M, N, tiles_n);
+    hipLaunchKernelGGL(gated_gradients_kernel<_Float16>, grid, dim3(256), 0, stream, (const _Float16*)dH, (const _Float16*)GU, (_Float16*)D, (_Float16*)DT, M, N, cols_d, cols_dt, tiles_n);
   return hipGetLastError();
 }
 

@@ -153,6 +153,9 @@ struct GemmParams {
   // kEpiPartialFused, measurement only: 1 = no reducing workgroups; the multiplying workgroup of (tile, slice s)
   // reduces parts s, s + splits, ... of its tile itself.  Every multiplying workgroup must then be resident at once.
   int sk_self;
+  // B stored [K][N]: its rows; behind the last one, up to K, come zeros (K is then a multiple of kBK and N of 8, the rows missing
+  // are fewer than kBK, and A's columns there are zeros as well: rows of A in whole lines whatever their number of columns)
+  int b_rows;
   void* gu;  // kEpiGated: 16-bit [M][2 N], the two factors before the activation; null: not asked for
 };
 
@@ -713,6 +716,7 @@ struct GemmTile {
         const int koff = tile_koff(t);
         int rows = klen - koff;
         if (rows > kBK) rows = kBK;
+        if (rows > p.b_rows - kb - koff) rows = p.b_rows - kb - koff;
         // (n_odd: another row of at least 8 elements follows every tile fetched here, so its last row may be read to a
         // whole chunk; the range check works on whole dwords and would cut an odd last column off)
         // (Whole lines: behind the last row that is multiplied here A's are zeros, and zero times infinity is not; one element

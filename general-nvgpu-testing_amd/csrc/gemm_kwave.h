@@ -34,6 +34,7 @@ struct KwParams {
   void* C;
   int M, N, K;
   int tiles_m, tiles_n, group_m;
+  int b_rows;  // as GemmParams::b_rows
   TileDivs divs;
 };
 
@@ -203,7 +204,8 @@ struct KwTile {
         const int koff = (t0 + (SHIFT ? t - 1 : t * EVERY)) * kBK;
         const bool exists = SHIFT ? t >= 1 && t <= n : t < n;
         // (not the rows behind the whole chunks: those of A are zeros there, and zero times infinity is not)
-        const int rows = 8 * k8 - koff < kBK ? 8 * k8 - koff : kBK;
+        const int end = 8 * k8 < p.b_rows ? 8 * k8 : p.b_rows;
+        const int rows = end - koff < kBK ? end - koff : kBK;
         // (columns past N in the rows in front of the last read the next row's data and feed outputs that do not exist)
         // The range check works on whole dwords from a lane's own offset: an odd last column needs the element behind it in range,
         // and that one alone is no whole dword of the row behind, which starts there.  (Telling the lanes of that row instead, by

@@ -250,7 +250,7 @@ struct GemmW4 {
       // [K][N]: the tile's columns of all K rows (the range check counts the scalar offset, which holds the K
       // tile here, together with the per-lane one).  Columns past the tile's last one read the next row's data,
       // past the last row's end nothing: they only feed output columns that do not exist.
-      if constexpr (B_KMAJOR) return make_rsrc((const T*)p.B + col0, ((unsigned)(K - 1) * (unsigned)N + (unsigned)rows) * 2u);
+      if constexpr (B_KMAJOR) return make_rsrc((const T*)p.B + col0, ((unsigned)(p.b_rows - 1) * (unsigned)N + (unsigned)rows) * 2u);
       return make_rsrc((const T*)p.B + (size_t)col0 * K, (unsigned)rows * (unsigned)K * 2u);
     };
     // A load stream: the operand rows of the output tile it is at (a finished buffer descriptor), the K

@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -167,10 +168,162 @@ PyObject* parallel_gemmrc_silu(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// ---- feed-forward operators.  They run on whatever GPU their tensors lie on; here only where that is the current one.
+
+int current_device() {
+  int d = -1;
+  return hipGetDevice(&d) == hipSuccess ? d : -1;
+}
+
+bool on_device(PyObject* o, int device) { return THPVariable_Unpack(o).device().index() == device; }
+
+// A 16-bit matrix on `device`.
+bool matrix(PyObject* o, int device, View* v) { return describe(o, v) && v->dims == 2 && v->size[0] <= INT_MAX && v->size[1] <= INT_MAX && on_device(o, device); }
+
+bool is_matrix(PyObject* o, int device, int dtype, int64_t rows, int64_t cols, View* v) {
+  return matrix(o, device, v) && v->dtype == dtype && v->size[0] == rows && v->size[1] == cols;
+}
+
+// Elements and scales in MXFP4 on `device`, and what they stand for.
+struct Held {
+  void* elements;
+  void* scales;
+  int64_t rows, cols;
+};
+bool held(PyObject* q, PyObject* s, int device, Held* h) {
+  if (!THPVariable_CheckExact(q) || !THPVariable_CheckExact(s)) return false;
+  const at::Tensor& e = THPVariable_Unpack(q);
+  const at::Tensor& t = THPVariable_Unpack(s);
+  for (const at::Tensor* x : {&e, &t})
+    if (!x->defined() || !x->is_cuda() || x->layout() != at::kStrided || !x->is_contiguous() || x->scalar_type() != at::kByte || x->device().index() != device) return false;
+  if (e.dim() != 2 || t.dim() != 3 || e.size(0) > INT_MAX / 4 || e.size(1) > INT_MAX / 4) return false;
+  h->rows = e.size(0);
+  h->cols = 2 * e.size(1);
+  h->elements = e.data_ptr();
+  h->scales = t.data_ptr();
+  return h->cols % 32 == 0 && t.size(0) == (h->cols + 255) / 256 && t.size(1) == h->rows && t.size(2) == 8;
+}
+
+// Workspace of one call, from torch's allocator: it goes back when the call returns, to calls behind it on its stream.
+c10::DataPtr call_workspace(size_t bytes) { return bytes ? c10::hip::HIPCachingAllocator::get()->allocate(bytes) : c10::DataPtr(); }
+
+// (a, b, h, gu or None)
+PyObject* gemmrc_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return status_of([&]() -> long {
+    View a, b, h, gu;
+    const int dev = current_device();
+    if (n != 4 || !matrix(args[0], dev, &a) || !matrix(args[1], dev, &b)) return kNotHandled;
+    const int64_t M = a.size[0], K = a.size[1], N2 = b.size[0];
+    if (b.dtype != a.dtype || b.size[1] != K || N2 % 2 != 0 || !is_matrix(args[2], dev, a.dtype, M, N2 / 2, &h)) return kNotHandled;
+    const bool train = args[3] != Py_None;
+    if (train && !is_matrix(args[3], dev, a.dtype, M, N2, &gu)) return kNotHandled;
+    void* const stream = c10::hip::getCurrentHIPStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = beam_gemmrc_gated(a.ptr, b.ptr, h.ptr, train ? gu.ptr : nullptr, (int)M, (int)(N2 / 2), (int)K, a.dtype, stream);
+    Py_END_ALLOW_THREADS;
+    return rc;
+  });
+}
+
+// (dh, gu, a, b, da or None, db or None)
+PyObject* gemmrc_gated_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return status_of([&]() -> long {
+    View dh, gu, a, b, da, db;
+    const int dev = current_device();
+    if (n != 6 || !matrix(args[2], dev, &a) || !matrix(args[3], dev, &b)) return kNotHandled;
+    const int64_t M = a.size[0], K = a.size[1], N2 = b.size[0];
+    if (b.dtype != a.dtype || b.size[1] != K || N2 % 2 != 0) return kNotHandled;
+    if (!is_matrix(args[0], dev, a.dtype, M, N2 / 2, &dh) || !is_matrix(args[1], dev, a.dtype, M, N2, &gu)) return kNotHandled;
+    const bool want_a = args[4] != Py_None, want_b = args[5] != Py_None;
+    if ((want_a && !is_matrix(args[4], dev, a.dtype, M, K, &da)) || (want_b && !is_matrix(args[5], dev, a.dtype, N2, K, &db))) return kNotHandled;
+    void* const stream = c10::hip::getCurrentHIPStream().stream();
+    const size_t bytes = beam_gemmrc_gated_backward_workspace_bytes((int)M, (int)(N2 / 2), want_a, want_b);
+    const c10::DataPtr ws = call_workspace(bytes);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = beam_gemmrc_gated_backward(dh.ptr, gu.ptr, a.ptr, b.ptr, want_a ? da.ptr : nullptr, want_b ? db.ptr : nullptr, (int)M, (int)(N2 / 2), (int)K,
+                                    a.dtype, ws.get(), bytes, stream);
+    Py_END_ALLOW_THREADS;
+    return rc;
+  });
+}
+
+// (x, q, scales)
+PyObject* mxfp4_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return status_of([&]() -> long {
+    View x;
+    Held h;
+    const int dev = current_device();
+    if (n != 3 || !matrix(args[0], dev, &x) || !held(args[1], args[2], dev, &h) || x.size[0] != h.rows || x.size[1] != h.cols) return kNotHandled;
+    void* const stream = c10::hip::getCurrentHIPStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = beam_mxfp4_quantize(x.ptr, h.elements, h.scales, (int)h.rows, (int)h.cols, x.dtype, stream);
+    Py_END_ALLOW_THREADS;
+    return rc;
+  });
+}
+
+// (q, scales, x)
+PyObject* mxfp4_dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return status_of([&]() -> long {
+    View x;
+    Held h;
+    const int dev = current_device();
+    if (n != 3 || !matrix(args[2], dev, &x) || !held(args[0], args[1], dev, &h) || x.size[0] != h.rows || x.size[1] != h.cols) return kNotHandled;
+    void* const stream = c10::hip::getCurrentHIPStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = beam_mxfp4_dequantize(h.elements, h.scales, x.ptr, (int)h.rows, (int)h.cols, x.dtype, stream);
+    Py_END_ALLOW_THREADS;
+    return rc;
+  });
+}
+
+// (a, a_scales, b, b_scales, c)
+PyObject* gemmrc_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return status_of([&]() -> long {
+    View c;
+    Held a, b;
+    const int dev = current_device();
+    if (n != 5 || !held(args[0], args[1], dev, &a) || !held(args[2], args[3], dev, &b) || a.cols != b.cols || !matrix(args[4], dev, &c)) return kNotHandled;
+    if (c.size[0] != a.rows || c.size[1] != b.rows) return kNotHandled;
+    void* const stream = c10::hip::getCurrentHIPStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = beam_gemmrc_mxfp4(a.elements, a.scales, b.elements, b.scales, c.ptr, (int)a.rows, (int)b.rows, (int)a.cols, c.dtype, stream);
+    Py_END_ALLOW_THREADS;
+    return rc;
+  });
+}
+
+// (a, b, b_scales, c)
+PyObject* linear_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return status_of([&]() -> long {
+    View a, c;
+    Held b;
+    const int dev = current_device();
+    if (n != 4 || !matrix(args[0], dev, &a) || !held(args[1], args[2], dev, &b) || a.size[1] != b.cols) return kNotHandled;
+    if (!is_matrix(args[3], dev, a.dtype, a.size[0], b.rows, &c)) return kNotHandled;
+    void* const stream = c10::hip::getCurrentHIPStream().stream();
+    const size_t bytes = beam_linear_mxfp4_workspace_bytes((int)a.size[0], (int)b.cols);
+    const c10::DataPtr ws = call_workspace(bytes);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS;
+    rc = beam_linear_mxfp4(a.ptr, b.elements, b.scales, c.ptr, (int)a.size[0], (int)b.rows, (int)b.cols, a.dtype, ws.get(), bytes, stream);
+    Py_END_ALLOW_THREADS;
+    return rc;
+  });
+}
+
 #define BEAM_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {BEAM_METHOD(gemmrc),    BEAM_METHOD(matmul),
                           BEAM_METHOD(gemmrc_splitk), BEAM_METHOD(gemmrc_ln),
-                          BEAM_METHOD(parallel_gemmrc_silu), {nullptr, nullptr, 0, nullptr}};
+                          BEAM_METHOD(parallel_gemmrc_silu),
+                          BEAM_METHOD(gemmrc_gated), BEAM_METHOD(gemmrc_gated_backward),
+                          BEAM_METHOD(mxfp4_quantize), BEAM_METHOD(mxfp4_dequantize),
+                          BEAM_METHOD(gemmrc_mxfp4), BEAM_METHOD(linear_mxfp4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
