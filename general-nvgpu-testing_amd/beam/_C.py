@@ -142,6 +142,7 @@ def _load() -> ctypes.CDLL:
     L.beam_dbg_ln_plan_bytes.restype = sz
     L.beam_dbg_assume_compute_units.argtypes = [i]
     L.beam_dbg_small_tile.argtypes = [i, i, i, i, i] + [ctypes.POINTER(i)] * 4
+    L.beam_dbg_set_mx_tile.argtypes = L.beam_dbg_set_gated_tile.argtypes = [i, i, i]
     L.beam_dbg_mx_tile.argtypes = [i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_gated_tile.argtypes = [i, i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_nn_off_lines_tile.argtypes = [i, i, i, cfgp, cfgp, ctypes.POINTER(i)]

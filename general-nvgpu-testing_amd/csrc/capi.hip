@@ -1018,7 +1018,12 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
 namespace {
 
 // The tile of gemm_kwave.h for a gated layer, if any; as kw_plan for its 2 N rows of B, of which the tiles here have 32 or 64.
+std::atomic<int> g_gated_rows{0}, g_gated_cols{0}, g_gated_kind{0};  // beam_dbg_set_gated_tile
 KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
+  if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) {
+    const int kind = g_gated_kind.load(std::memory_order_relaxed);
+    return kind < 4 ? KwPlan{0, 0, 0, false} : KwPlan{forced, g_gated_cols.load(std::memory_order_relaxed), 4, kind == 5};
+  }
   static const struct { int rows, cols; } kTiles[] = {{8, 32}, {16, 32}, {32, 32}, {8, 64}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
   const KwPlan none = {0, 0, 0, false};
   if (K < 8 || K > kMaxK) return none;
@@ -1037,6 +1042,7 @@ KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
 
 // The tile of the gated kernel: what beam_gemmrc would take for the 2 N rows of B, as far as there is one like it.
 GatedTile gated_tile(int M, int N, int K, RowStarts rows, int cus) {
+  if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) return GatedTile{forced, g_gated_cols.load(std::memory_order_relaxed), g_gated_kind.load(std::memory_order_relaxed)};
   if (K % kBK != 0 && rows == kOnChunks) {
     const LineChoice t = off_lines_tile(M, 2 * N, K, cus);
     if (t.lines) return GatedTile{t.cfg.block_m == 128 && t.cfg.block_n == 64 ? 64 : t.cfg.block_m, 128, kGatedLines};
@@ -1169,23 +1175,39 @@ int check_mx_product(const void* C, int M, int N, int K, int dtype) {
 // What an MXFP4 product runs on: rows x cols, the tile of gemm_mx.h's two kernels.
 struct MxPlan {
   int rows, cols;
-  bool kwave;
+  int kwave;  // 1: K tiles dealt out to the wavefronts; 2: the kernel of gemm_w4.h
 };
-MxPlan mx_plan(int M, int N, int cus) {
+std::atomic<int> g_mx_rows{0}, g_mx_cols{0}, g_mx_kwave{0};  // beam_dbg_set_mx_tile
+MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
+  if (const int rows = g_mx_rows.load(std::memory_order_relaxed)) return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), g_mx_kwave.load(std::memory_order_relaxed)};
   static const struct { int rows, cols; } kSmall[] = {{16, 16}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
   auto tiles = [&](int r, int c) { return ((long)M + r - 1) / r * (((long)N + c - 1) / c); };
   for (const auto& t : kSmall) {
     const bool few = M <= 16 && t.rows == 16 && t.cols == 64;
-    if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, true};
+    if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, 1};
   }
-  if (tiles(256, 256) >= cus) return MxPlan{256, 256, false};
-  if (tiles(256, 128) >= cus) return MxPlan{256, 128, false};
-  if (tiles(128, 128) >= cus) return MxPlan{128, 128, false};
-  return MxPlan{64, 64, false};
+  const bool w4_fits = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
+  if (tiles(256, 256) >= cus) return MxPlan{256, 256, w4_fits ? 2 : 0};
+  if (tiles(256, 128) >= cus) return MxPlan{256, 128, 0};
+  if (tiles(128, 128) >= cus) return MxPlan{128, 128, 0};
+  return MxPlan{64, 64, 0};
 }
 
 int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* sB, void* C, int M, int N, int K, int dtype, hipStream_t st) {
-  const MxPlan plan = mx_plan(M, N, g_dev.cus > 0 ? g_dev.cus : 256);
+  const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
+  const MxPlan plan = mx_plan(M, N, K, C, cus);
+  if (plan.kwave == 2) {
+    const beam_tile_cfg c = {256, 256, 128, 128, 0, default_group_m(256, 256)};
+    MxW4Params p;
+    static_cast<GemmParams&>(p) = base_params(A, B, M, N, K / 4, c);
+    p.C = C;
+    p.sa = (const uint8_t*)sA;
+    p.sb = (const uint8_t*)sB;
+    p.c_store = (size_t)M * N * 2 >= ((size_t)256 << 20) && K >= 4096 ? kStoreStreaming : store_kind(c, 4, true, C, M, N, K);
+    const long tiles = (long)p.tiles_m * p.tiles_n;
+    BEAM_HIP(launch_gemm_mx_w4(p, dtype, dim3((unsigned)(tiles < cus ? tiles : cus)), st));
+    return BEAM_OK;
+  }
   MxParams p;
   p.A = A;
   p.B = B;
@@ -2070,9 +2092,25 @@ int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, 
   return BEAM_OK;
 }
 
+int beam_dbg_set_mx_tile(int rows, int cols, int kwave) {
+  g_mx_rows.store(0);
+  g_mx_cols.store(cols);
+  g_mx_kwave.store(kwave);
+  g_mx_rows.store(rows);
+  return BEAM_OK;
+}
+
+int beam_dbg_set_gated_tile(int rows, int cols, int kind) {
+  g_gated_rows.store(0);
+  g_gated_cols.store(cols);
+  g_gated_kind.store(kind);
+  g_gated_rows.store(rows);
+  return BEAM_OK;
+}
+
 int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave) {
   if (!rows || !cols || !kwave || M < 1 || N < 1 || K < 32) return fail(BEAM_ERR_INVALID, "arguments");
-  const MxPlan plan = mx_plan(M, N, g_dev.cus > 0 ? g_dev.cus : 256);
+  const MxPlan plan = mx_plan(M, N, K, nullptr, g_dev.cus > 0 ? g_dev.cus : 256);
   *rows = plan.rows, *cols = plan.cols, *kwave = plan.kwave;
   return BEAM_OK;
 }

@@ -14,19 +14,37 @@
 
 namespace beam {
 
-// The scales of NB blocks of 16 rows for one K tile, read from the 8 bytes a row at `first` (this lane's two bytes of block 0):
-// lane (r, g) has those of row r, chunks 2 g and 2 g + 1; two blocks to a register.
+// The scales of NB blocks of 16 rows for one K tile in a lane (r, g): those of row r of each block, chunks 2 g and 2 g + 1, 16
+// bits, two blocks to a register.
 template <int NB>
 struct MxScales {
+  static constexpr bool QUADS = NB % 4 == 0;
   static constexpr int REGS = (NB + 1) / 2;
   int reg[REGS];
+  static constexpr int reg_of(int i) { return QUADS ? 2 * (i >> 2) + (i & 1) : i >> 1; }
+  static constexpr int half_of(int i) { return QUADS ? (i >> 1) & 1 : i & 1; }
 
-  __device__ __forceinline__ void read(const char* first) {
+  // The rows' 8 bytes lie side by side from `rows` on.  Four blocks are 64 rows: lane (r, g) reads the 8 bytes of row r of block g
+  // at once, and the four lane groups exchange what they need of each other's (mx_turn); otherwise the 16 bits of each block.
+  i32x2 raw[QUADS ? NB / 4 : 1];
+  __device__ __forceinline__ void read(const char* rows, int lane) {
+    if constexpr (QUADS) {
 #pragma unroll
-    for (int i = 0; i < REGS; ++i) {
-      const int lo = *(const unsigned short*)(first + 2 * i * 128);
-      const int hi = 2 * i + 1 < NB ? (int)*(const unsigned short*)(first + (2 * i + 1) * 128) : 0;
-      reg[i] = lo | hi << 16;
+      for (int q = 0; q < NB / 4; ++q) raw[q] = *(const i32x2*)(rows + q * 512 + lane * 8);
+    } else {
+      const char* const first = rows + (lane & 15) * kMxBlocks + 2 * (lane >> 4);
+#pragma unroll
+      for (int i = 0; i < REGS; ++i) {
+        const int lo = *(const unsigned short*)(first + 2 * i * 128);
+        const int hi = 2 * i + 1 < NB ? (int)*(const unsigned short*)(first + (2 * i + 1) * 128) : 0;
+        reg[i] = lo | hi << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void turn() {
+    if constexpr (QUADS) {
+#pragma unroll
+      for (int q = 0; q < NB / 4; ++q) mx_turn(raw[q], &reg[2 * q], &reg[2 * q + 1]);
     }
   }
   __device__ __forceinline__ void mask(int m) {
@@ -43,20 +61,26 @@ __device__ __forceinline__ int mx_tail_mask(int blocks, int g) {
   return m | m << 16;
 }
 
-// acc[i][j] += step KK of blocks i of A and j of B.
-template <int KK, int FM, int FN>
-__device__ __forceinline__ void mx_multiply(const i32x4 (&fa)[FM], const i32x4 (&fb)[FN], const MxScales<FM>& sa, const MxScales<FN>& sb,
-                                            f32x4 (&acc)[FM][FN]) {
+// acc[j] += step KK of block I of A and blocks j of B.
+template <int KK, int I, int FM, int FN>
+__device__ __forceinline__ void mx_multiply_row(i32x4 fa, const i32x4 (&fb)[FN], const MxScales<FM>& sa, const MxScales<FN>& sb, f32x4 (&acc)[FN]) {
+  using A = MxScales<FM>;
+  using B = MxScales<FN>;
+  const int s_a = sa.reg[A::reg_of(I)];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int s_b = sb.reg[j >> 1], s_a = sa.reg[i >> 1];
-      if ((j & 1) == 0 && (i & 1) == 0) acc[i][j] = mx_mfma<KK, 0, 0>(fb[j], fa[i], acc[i][j], s_b, s_a);
-      else if ((j & 1) == 0) acc[i][j] = mx_mfma<KK, 0, 1>(fb[j], fa[i], acc[i][j], s_b, s_a);
-      else if ((i & 1) == 0) acc[i][j] = mx_mfma<KK, 1, 0>(fb[j], fa[i], acc[i][j], s_b, s_a);
-      else acc[i][j] = mx_mfma<KK, 1, 1>(fb[j], fa[i], acc[i][j], s_b, s_a);
-    }
+  for (int j = 0; j < FN; ++j) {
+    if (B::half_of(j) == 0) acc[j] = mx_mfma<KK, 0, A::half_of(I)>(fb[j], fa, acc[j], sb.reg[B::reg_of(j)], s_a);
+    else acc[j] = mx_mfma<KK, 1, A::half_of(I)>(fb[j], fa, acc[j], sb.reg[B::reg_of(j)], s_a);
+  }
+}
+
+// f(0), ..., f(N - 1) with the index as a constant.
+template <int I, int N, typename F>
+__device__ __forceinline__ void mx_static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    mx_static_for<I + 1, N>(f);
+  }
 }
 
 // One fill of 1 KiB (8 rows of 128 bytes) or of 256 bytes (the scales of 32 rows) by a wavefront.
@@ -84,21 +108,28 @@ __device__ __forceinline__ void mx_store_quad(T* row, int n, int N, f32x4 v) {
 }
 
 // Workgroup tile BM x BN of WVM x WVN wavefronts that share a ring of ST LDS slots.
+//
+// The K loop is gemm_kernel.h's: while the MFMAs of one half of a K tile run, the fragments of the next half are read, a few
+// between the MFMAs of each row, and the fills of the K tile ST - 1 further on are issued, a row's share behind each row; of two
+// wavefronts on a SIMD the older one issues all of them.  A row is closed by a scheduling fence: left alone, the compiler reads
+// every fragment right in front of the MFMA that needs it (MEASURED_PIPELINE).
 template <typename T, int BM, int BN, int WVM, int WVN, int ST>
 struct MxGemm {
   static constexpr int NW = WVM * WVN, NT = NW * 64;
+  static constexpr int LDW = NW >= 8 ? NW / 2 : NW, NTL = LDW * 64;  // wavefronts that fill LDS, their threads
   static constexpr int TM = BM / WVM, TN = BN / WVN;
   static constexpr int FM = TM / 16, FN = TN / 16;
   static constexpr int A_BYTES = BM * kRowBytes, B_BYTES = BN * kRowBytes;
   static constexpr int SCALES = A_BYTES + B_BYTES;  // where a slot's scales begin: A's, then B's
-  static constexpr int LS = ((BM + BN) / 32 + NW - 1) / NW;  // fills of scales by a wavefront
-  static constexpr int SLOT = SCALES + LS * NW * 256;
+  static constexpr int LS = ((BM + BN) / 32 + LDW - 1) / LDW;  // fills of scales by a loader
+  static constexpr int SLOT = SCALES + LS * LDW * 256;
   static constexpr int LDS_BYTES = ST * SLOT;
-  static constexpr int LA = BM * kChunksPerRow / NT, LB = BN * kChunksPerRow / NT;
+  static constexpr int LA = BM * kChunksPerRow / NTL, LB = BN * kChunksPerRow / NTL;
   static constexpr int LOADS = LA + LB + LS;
   static constexpr int WAIT = (ST - 2) * LOADS;  // fills behind those of the K tile that is waited for
+  static constexpr int PER_ROW = (LOADS + 2 * FM - 1) / (2 * FM);
   static_assert(LDS_BYTES <= 160 * 1024 && WAIT < 64 && ST >= 2, "LDS, vmcnt range");
-  static_assert(BM * kChunksPerRow % NT == 0 && BN * kChunksPerRow % NT == 0 && BM % 32 == 0 && BN % 32 == 0, "whole fills");
+  static_assert(BM * kChunksPerRow % NTL == 0 && BN * kChunksPerRow % NTL == 0 && BM % 32 == 0 && BN % 32 == 0, "whole fills");
 
   static __device__ __forceinline__ void run(const MxParams& p, char* smem) {
     const int tid = threadIdx.x, lane = tid & 63;
@@ -119,36 +150,39 @@ struct MxGemm {
     unsigned voff_a[LA], voff_b[LB];
 #pragma unroll
     for (int i = 0; i < (LA > LB ? LA : LB); ++i) {
-      const int q = i * NT + tid, row = q >> 3;
-      const unsigned off = (unsigned)row * row_bytes + (unsigned)(((q & 7) ^ swizzle_of_row(row)) << 4);
+      const int q = i * NTL + tid, row = q >> 3;
+      const unsigned off = (unsigned)row * row_bytes + (unsigned)(mx_chunk_at((q & 7) ^ swizzle_of_row(row)) << 4);
       if (i < LA) voff_a[i] = off;
       if (i < LB) voff_b[i] = off;
     }
     const char* const a_base = (const char*)p.A + (size_t)row0 * row_bytes;
     const char* const b_base = (const char*)p.B + (size_t)col0 * row_bytes;
-    auto fill = [&](int t, char* slot) __attribute__((always_inline)) {
+    // fill l of K tile t: B's rows, A's, the scales
+    auto fill = [&](int l, int t, char* slot) __attribute__((always_inline)) {
       const bool there = t < n_tiles;
       const unsigned koff = there ? (unsigned)t * kRowBytes : 0u;
-      const __amdgpu_buffer_rsrc_t ra = make_rsrc(a_base, there ? (unsigned)rows_a * row_bytes : 0u);
-      const __amdgpu_buffer_rsrc_t rb = make_rsrc(b_base, there ? (unsigned)rows_b * row_bytes : 0u);
-#pragma unroll
-      for (int i = 0; i < LA; ++i) mx_fill_rows(ra, slot + i * (NT * 16) + wave * 1024, voff_a[i] + koff);
-#pragma unroll
-      for (int i = 0; i < LB; ++i) mx_fill_rows(rb, slot + A_BYTES + i * (NT * 16) + wave * 1024, voff_b[i] + koff);
-      const size_t kt = there ? (size_t)t : 0;
-#pragma unroll
-      for (int i = 0; i < LS; ++i) {
-        const int part = i * NW + wave;  // of 32 rows; A's come first (and behind B's there may be an empty one)
+      if (l < LB) {
+        mx_fill_rows(make_rsrc(b_base, there ? (unsigned)rows_b * row_bytes : 0u), slot + A_BYTES + l * (NTL * 16) + wave * 1024, voff_b[l] + koff);
+      } else if (l < LB + LA) {
+        const int i = l - LB;
+        mx_fill_rows(make_rsrc(a_base, there ? (unsigned)rows_a * row_bytes : 0u), slot + i * (NTL * 16) + wave * 1024, voff_a[i] + koff);
+      } else {
+        const int part = (l - LB - LA) * LDW + wave;  // of 32 rows; A's come first (and behind B's there may be an empty one)
         const bool of_a = part < BM / 32;
+        const size_t kt = there ? (size_t)t : 0;
         const uint8_t* const base = of_a ? p.sa + (kt * M + row0) * kMxBlocks : p.sb + (kt * N + col0) * kMxBlocks;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(base, there && part < (BM + BN) / 32 ? (unsigned)(of_a ? rows_a : rows_b) * kMxBlocks : 0u);
         mx_fill_scales(rs, slot + SCALES + part * 256, (unsigned)(of_a ? part : part - BM / 32) * 256u + (unsigned)lane * 4u);
       }
     };
-    const int tail_mask = mx_tail_mask(p.K / 32 - (n_tiles - 1) * kMxBlocks, g);
-
+    const bool loader = LDW == NW || wave < LDW;
+    if (loader) {
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) fill(s, smem + s * SLOT);
+      for (int s = 0; s < ST - 1; ++s)
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) fill(l, s, smem + s * SLOT);
+    }
+    const int tail_mask = mx_tail_mask(p.K / 32 - (n_tiles - 1) * kMxBlocks, g);
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -156,35 +190,85 @@ struct MxGemm {
       for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int frag_off[2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) frag_off[kk] = lds_offset(r, 2 * g + kk);
-    const int scale_a = SCALES + (wm * TM + r) * kMxBlocks + 2 * g, scale_b = SCALES + (BM + wn * TN + r) * kMxBlocks + 2 * g;
+    for (int kk = 0; kk < 2; ++kk) frag_off[kk] = lds_offset(r, 4 * kk + g);
+    const int wave_a = wm * TM * kRowBytes, wave_b = A_BYTES + wn * TN * kRowBytes;
+    const int wave_sa = SCALES + wm * TM * kMxBlocks, wave_sb = SCALES + (BM + wn * TN) * kMxBlocks;
 
-    char* now = smem;
-    char* next = smem + (ST - 1) * SLOT;  // the slot that K tile h - 1 was in
-    for (int h = 0; h < n_tiles; ++h) {
-      wait_vm_and_lds<WAIT>();
-      bare_barrier();  // everyone's fills of K tile h are there, and everyone has read K tile h - 1
-      fill(h + ST - 1, next);
-      MxScales<FM> sa;
-      MxScales<FN> sb;
-      sa.read(now + scale_a);
-      sb.read(now + scale_b);
-      if (h == n_tiles - 1) sa.mask(tail_mask), sb.mask(tail_mask);
-      const char* const at_a = now + wm * TM * kRowBytes;
-      const char* const at_b = now + A_BYTES + wn * TN * kRowBytes;
-      i32x4 fa[2][FM], fb[2][FN];
+    // Fragments of the halves of a K tile, and their scales: zeros to begin with, so that the first step multiplies nothing.
+    i32x4 fa0[FM], fa1[FM], fb0[FN], fb1[FN];
+    MxScales<FM> sa;
+    MxScales<FN> sb;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
+    for (int i = 0; i < FM; ++i) fa1[i] = i32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[kk][j] = *(const i32x4*)(at_b + j * 16 * kRowBytes + frag_off[kk]);
+    for (int j = 0; j < FN; ++j) fb1[j] = i32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < FM; ++i) fa[kk][i] = *(const i32x4*)(at_a + i * 16 * kRowBytes + frag_off[kk]);
+    for (int i = 0; i < MxScales<FM>::REGS; ++i) sa.reg[i] = 0;
+#pragma unroll
+    for (int j = 0; j < MxScales<FN>::REGS; ++j) sb.reg[j] = 0;
+    // Multiplies half KK with (ca, cb), reads the next half (na, nb) and issues the fills of rows ROW0 .. of K tile h + ST - 1.
+    auto step = [&](auto kk_tag, auto row0_tag, auto ld_tag, const i32x4(&ca)[FM], const i32x4(&cb)[FN], i32x4(&na)[FM], i32x4(&nb)[FN], const char* slot,
+                    int off, int h, char* fill_slot) __attribute__((always_inline)) {
+      constexpr int KK = decltype(kk_tag)::value, ROW0 = decltype(row0_tag)::value;
+      constexpr bool LD = decltype(ld_tag)::value;
+      constexpr int READS = FM + FN, READ_ROWS = FM > 1 ? FM - 1 : 1, PER_READ_ROW = (READS + READ_ROWS - 1) / READ_ROWS;
+      mx_static_for<0, FM>([&](auto i_tag) __attribute__((always_inline)) {
+        constexpr int i = decltype(i_tag)::value;
+#pragma unroll
+        for (int u = 0; u < PER_READ_ROW; ++u) {
+          const int n = i * PER_READ_ROW + u;
+          if (i < READ_ROWS && n < READS) {
+            if (n < FN) nb[n] = *(const i32x4*)(slot + wave_b + n * 16 * kRowBytes + off);
+            else na[n - FN] = *(const i32x4*)(slot + wave_a + (n - FN) * 16 * kRowBytes + off);
+          }
+        }
+        mx_multiply_row<KK, i>(ca[i], cb, sa, sb, acc[i]);
+        if constexpr (LD) {
+#pragma unroll
+          for (int u = 0; u < PER_ROW; ++u)
+            if ((ROW0 + i) * PER_ROW + u < LOADS) fill((ROW0 + i) * PER_ROW + u, h + ST - 1, fill_slot);
+        }
+        if constexpr (FN >= 4) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x020, PER_ROW, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, FN - 3, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    auto loop = [&](auto ld_tag) __attribute__((always_inline)) {
+      constexpr bool LD = decltype(ld_tag)::value;
+      char* now = smem;
+      char* free = smem + (ST - 1) * SLOT;  // the slot that K tile h - 1 was in
+      for (int h = 0; h < n_tiles; ++h) {
+        // my fills of K tile h are there, my reads of K tile h - 1 done ...
+        if constexpr (LD) wait_vm_and_lds<WAIT>();
+        else wait_lds<0>();
+        bare_barrier();  // ... and everyone's
+        MxScales<FM> ta;
+        MxScales<FN> tb;
+        ta.read(now + wave_sa, lane);
+        tb.read(now + wave_sb, lane);
+        step(std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{}, ld_tag, fa1, fb1, fa0, fb0, now, frag_off[0], h, free);
+        ta.turn();
+        tb.turn();
+        if (h == n_tiles - 1) ta.mask(tail_mask), tb.mask(tail_mask);
+        sa = ta, sb = tb;
+        step(std::integral_constant<int, 0>{}, std::integral_constant<int, FM>{}, ld_tag, fa0, fb0, fa1, fb1, now, frag_off[1], h, free);
+        free = now;
+        now = now + SLOT == smem + ST * SLOT ? smem : now + SLOT;
       }
-      mx_multiply<0>(fa[0], fb[0], sa, sb, acc);
-      mx_multiply<1>(fa[1], fb[1], sa, sb, acc);
-      next = now;
-      now = now + SLOT == smem + ST * SLOT ? smem : now + SLOT;
-    }
+    };
+    if (loader) loop(std::true_type{});
+    else loop(std::false_type{});
+    mx_static_for<0, FM>([&](auto i_tag) __attribute__((always_inline)) {  // the second half of the last K tile
+      mx_multiply_row<1, decltype(i_tag)::value>(fa1[decltype(i_tag)::value], fb1, sa, sb, acc[decltype(i_tag)::value]);
+    });
     wait_vm_and_lds<0>();  // (fills behind the last K tile)
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -246,7 +330,7 @@ struct MxKw {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int row = 8 * c + (lane >> 3);
-      voff[c] = (unsigned)row * row_bytes + (unsigned)(((lane & 7) ^ swizzle_of_row(row)) << 4);
+      voff[c] = (unsigned)row * row_bytes + (unsigned)(mx_chunk_at((lane & 7) ^ swizzle_of_row(row)) << 4);
     }
     const char* const a_base = (const char*)p.A + (size_t)row0 * row_bytes;  // (not A16)
     const char* const b_base = (const char*)p.B + (size_t)col0 * row_bytes;
@@ -293,7 +377,7 @@ struct MxKw {
         int scale;
         const i32x4 elements = mx_encode_block(x, &scale);
         char* const tile = kept + (b >> 3) * KEPT;
-        *(i32x4*)(tile + lds_offset(row, b & 7)) = elements;
+        *(i32x4*)(tile + lds_offset(row, mx_place_of(b & 7))) = elements;
         tile[A_BYTES + row * kMxBlocks + (b & 7)] = (char)scale;
       };
       vec8 x[4];
@@ -316,8 +400,7 @@ struct MxKw {
       for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int frag_off[2];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) frag_off[kk] = lds_offset(r, 2 * g + kk);
-    const int scale_off = r * kMxBlocks + 2 * g;
+    for (int kk = 0; kk < 2; ++kk) frag_off[kk] = lds_offset(r, 4 * kk + g);
     const int tail_mask = mx_tail_mask(K / 32 - (n_tiles - 1) * kMxBlocks, g);
     char* slot = ring;
     for (int t = 0; t < n; ++t) {
@@ -329,8 +412,8 @@ struct MxKw {
       i32x4 fa[2][MB], fb[2][CB];
       MxScales<MB> sa;
       MxScales<CB> sb;
-      sa.read(at_a + A_BYTES + scale_off);
-      sb.read(at_b + B_BYTES + scale_off);
+      sa.read(at_a + A_BYTES, lane);
+      sb.read(at_b + B_BYTES, lane);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
@@ -343,9 +426,14 @@ struct MxKw {
       __builtin_amdgcn_sched_barrier(0);
       fill(t + S, slot);
       __builtin_amdgcn_sched_barrier(0);
+      sa.turn();
+      sb.turn();
       if (wave + t * NW == n_tiles - 1) sa.mask(tail_mask), sb.mask(tail_mask);
-      mx_multiply<0>(fa[0], fb[0], sa, sb, acc);
-      mx_multiply<1>(fa[1], fb[1], sa, sb, acc);
+      mx_static_for<0, MB>([&](auto i_tag) __attribute__((always_inline)) {
+        constexpr int i = decltype(i_tag)::value;
+        mx_multiply_row<0, i>(fa[0][i], fb[0], sa, sb, acc[i]);
+        mx_multiply_row<1, i>(fa[1][i], fb[1], sa, sb, acc[i]);
+      });
       slot = slot + SLOT == ring + S * SLOT ? ring : slot + SLOT;
     }
     wait_vm_and_lds<0>();  // the empty fills of the last iterations must be gone before the rings are reused,

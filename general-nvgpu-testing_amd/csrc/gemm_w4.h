@@ -41,6 +41,7 @@
 #pragma once
 
 #include "gemm_kernel.h"
+#include "mx.h"
 
 namespace beam {
 
@@ -76,6 +77,20 @@ struct W4Mfma<__bf16> {
   template <int BLK>
   static __device__ __forceinline__ void first(bf16x8 b, bf16x8 a) {
     asm volatile("v_mfma_f32_16x16x32_bf16 a[%2:%3], %0, %1, 0" ::"v"(b), "v"(a), "n"(4 * BLK), "n"(4 * BLK + 3));
+  }
+};
+
+// The same of two MXFP4 operands (mx.h): chunk step STEP of a K tile, halves HB and HA of the scale registers.
+struct W4MxMfma {
+  template <int BLK, int STEP, int HB, int HA>
+  static __device__ __forceinline__ void fma(i32x4 b, i32x4 a, int scale_b, int scale_a) {
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 a[%4:%5], %0, %1, a[%4:%5], %2, %3 op_sel:[%6,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4" ::"v"(b), "v"(a),
+                 "v"(scale_b), "v"(scale_a), "n"(4 * BLK), "n"(4 * BLK + 3), "n"(STEP), "n"(HB), "n"(HA));
+  }
+  template <int BLK, int STEP, int HB, int HA>
+  static __device__ __forceinline__ void first(i32x4 b, i32x4 a, int scale_b, int scale_a) {
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 a[%4:%5], %0, %1, 0, %2, %3 op_sel:[%6,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4" ::"v"(b), "v"(a),
+                 "v"(scale_b), "v"(scale_a), "n"(4 * BLK), "n"(4 * BLK + 3), "n"(STEP), "n"(HB), "n"(HA));
   }
 };
 
@@ -143,9 +158,17 @@ __host__ __device__ inline int w4_b_row(int b, int r) { return 32 * (b >> 1) + 4
 // in the plain kernel -- the next tile's first operand tiles arrive while the band's statistics are
 // exchanged (walking_layer_norm below says why nobody waits for ever).
 // B_KMAJOR: B is stored [K][N].
-template <typename T, int STORE = kStoreThrough, bool LN = false, int SB = 4, int SA = 8, int G0 = 2, bool B_KMAJOR = false>
+// MX: A and B are MXFP4 (mx.h), T is C's type.  256 of their columns are the 128 bytes of a row that 64 16-bit elements are, so
+// the parameters' K is a quarter of theirs and everything that counts in 16-bit elements stands.  What differs is the MFMA, the
+// chunk of a K tile that a lane group takes in a step (mx_chunk_at), and the scales: a wavefront has two loads of each operand's for a K
+// tile, straight into registers (64 rows of 8 bytes each: MxScales' way of four blocks), asked for one K tile ahead behind the B
+// fills, exchanged between the lane groups while the K tile before is multiplied.  The fills are the compiler's builtins here: it
+// then knows that they are younger than the scales' loads and does not wait for all of them.
+template <typename T, int STORE = kStoreThrough, bool LN = false, int SB = 4, int SA = 8, int G0 = 2, bool B_KMAJOR = false, bool MX = false>
 struct GemmW4 {
   static_assert(!(LN && B_KMAJOR), "the fused LayerNorm is built for B as [N][K]");
+  static_assert(!(MX && (LN || B_KMAJOR)), "MXFP4 is built for the plain product");
+  using Params = std::conditional_t<MX, MxW4Params, GemmParams>;
   using Traits = ElemTraits<T>;
   using vec8 = typename Traits::vec8;
   using Mfma = W4Mfma<T>;
@@ -184,7 +207,7 @@ struct GemmW4 {
   static_assert(LAST_B + 3 < 64 && LAST_A + 3 < 64 && LAST_READ + 2 < LAST_A, "room for the scalar bookkeeping");
   static_assert(load_at(0, LAST_B) == LPT - 1 && load_at(1, LAST_A) == LPT - 1 && LAST_B < 62 && LAST_A < 62, "loads fit a step");
 
-  static __device__ __forceinline__ void run(const GemmParams& p, char* smem) {
+  static __device__ __forceinline__ void run(const Params& p, char* smem) {
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -224,13 +247,14 @@ struct GemmW4 {
 #pragma unroll
     for (int i = 0; i < LPT; ++i) {
       const unsigned row_bytes = (unsigned)(fill_row + 32 * i) * (unsigned)K * 2u;
-      voff_a[i] = row_bytes + (unsigned)(((lane & 7) ^ swizzle_of_row(fill_row)) << 4);
+      const int place_a = (lane & 7) ^ swizzle_of_row(fill_row), place_b = (lane & 7) ^ w4_swizzle_b(fill_row);
+      voff_a[i] = row_bytes + (unsigned)((MX ? mx_chunk_at(place_a) : place_a) << 4);
       if constexpr (B_KMAJOR) {
         // 1 KiB = rows k, k + 1 of the [K][N] tile, k = 8 i + 2 w; lane l fills position l % 32 of row k + l / 32
         const int k = 8 * i + 2 * wave + (lane >> 5);
         voff_b[i] = ((unsigned)k * (unsigned)N + (unsigned)(((lane & 31) ^ w4_kmajor_swizzle(k)) << 3)) * 2u;
       } else {
-        voff_b[i] = row_bytes + (unsigned)(((lane & 7) ^ w4_swizzle_b(fill_row)) << 4);
+        voff_b[i] = row_bytes + (unsigned)((MX ? mx_chunk_at(place_b) : place_b) << 4);
       }
     }
 
@@ -272,6 +296,7 @@ struct GemmW4 {
     // instruction.  The loads are therefore invisible to the compiler's wait-count bookkeeping; every wait
     // for them in this kernel is an explicit s_waitcnt vmcnt.
     auto set_load_target = [&](const Stream& st, auto i_tag) __attribute__((always_inline)) {
+      if constexpr (MX) return;
       // (the add writes the scalar condition bit: without that in the clobber list the compiler keeps a compare's
       // result alive across this statement and selects on the add's carry instead)
       asm volatile("s_add_u32 m0, %0, %1" ::"s"(st.lds), "n"(decltype(i_tag)::value * 4096) : "memory", "scc");
@@ -280,7 +305,12 @@ struct GemmW4 {
     // it) only 5 wait states later, which the compiler keeps for its own instructions and not in front of assembly.  So a stream's
     // first load behind a boundary of output tiles brings them along (FRESH: three in the prologue, two in a tile's first K tile; 8192 x
     // 8192 x 192, 4 tiles of 3 K tiles each, 54.8 us with and without).
-    auto load_tile_part = [&](const Stream& st, unsigned voff, auto fresh_tag) __attribute__((always_inline)) {
+    auto load_tile_part = [&](const Stream& st, unsigned voff, auto i_tag, auto fresh_tag) __attribute__((always_inline)) {
+      if constexpr (MX) {
+        char* const dst = smem + st.lds + decltype(i_tag)::value * 4096;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(st.rows, (__attribute__((address_space(3))) void*)dst, 16, (int)voff, st.koff, 0, 0);
+        return;
+      }
       if constexpr (decltype(fresh_tag)::value)
         asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(st.rows), "s"(st.koff) : "memory");
       else asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(st.rows), "s"(st.koff) : "memory");
@@ -336,6 +366,62 @@ struct GemmW4 {
         fb0[i][e] = 0;
         fb1[i][e] = 0;
       }
+
+    // ---- scales (MX) -----------------------------------------------------------------------------
+    // The stream of scales is one K tile ahead of the multiplication: K tile sc_kt of the rows from byte sc_a (sc_b) of K tile 0 on,
+    // sc_bytes_a (_b) of them; nothing behind the workgroup's last tile.
+    size_t sc_a = 0, sc_b = 0, next_sc_a = 0, next_sc_b = 0;
+    unsigned sc_bytes_a = 0, sc_bytes_b = 0, next_sc_bytes_a = 0, next_sc_bytes_b = 0;
+    int sc_kt = 0;
+    auto next_scales = [&](int j, TileCoord tc) __attribute__((always_inline)) {
+      const int row0 = tc.tm * BM, col0 = tc.tn * BN;
+      next_sc_a = (size_t)row0 * kMxBlocks;
+      next_sc_b = (size_t)col0 * kMxBlocks;
+      next_sc_bytes_a = j >= my_tiles ? 0u : (unsigned)(M - row0 < BM ? M - row0 : BM) * kMxBlocks;
+      next_sc_bytes_b = j >= my_tiles ? 0u : (unsigned)(N - col0 < BN ? N - col0 : BN) * kMxBlocks;
+    };
+    // lane (r, g) loads the 8 bytes of row r of blocks g (first load) and 4 + g (second)
+    const int sc_off_a = (wm * 128 + 16 * g + r) * kMxBlocks, sc_off_b = (wn * 128 + w4_b_row(g, r)) * kMxBlocks;
+    i32x2 raw[4];              // as loaded: two of A, two of B
+    int cur[8], nxt[8];        // of the K tiles whose second, and first, half is being multiplied: 4 registers of A, 4 of B
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cur[e] = nxt[e] = 0;
+    auto load_scales = [&](auto n_tag) __attribute__((always_inline)) {
+      if constexpr (!MX) return;
+      else {
+      constexpr int n = decltype(n_tag)::value;
+      __amdgpu_buffer_rsrc_t rows;
+      if constexpr (n < 2) rows = make_rsrc(p.sa + (sc_a + (size_t)sc_kt * M * kMxBlocks), sc_bytes_a);
+      else rows = make_rsrc(p.sb + (sc_b + (size_t)sc_kt * N * kMxBlocks), sc_bytes_b);
+      raw[n] = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(rows, (n < 2 ? sc_off_a : sc_off_b) + (n & 1) * 512, 0, 0));
+      }
+    };
+    auto turn_scales = [&](auto n_tag) __attribute__((always_inline)) {
+      constexpr int n = decltype(n_tag)::value;
+      mx_turn(raw[n], &nxt[2 * n], &nxt[2 * n + 1]);
+    };
+    auto advance_scales = [&]() __attribute__((always_inline)) {
+      const bool wrap = sc_kt + 1 == n_k;
+      sc_kt = wrap ? 0 : sc_kt + 1;
+      sc_a = wrap ? next_sc_a : sc_a;
+      sc_b = wrap ? next_sc_b : sc_b;
+      sc_bytes_a = wrap ? next_sc_bytes_a : sc_bytes_a;
+      sc_bytes_b = wrap ? next_sc_bytes_b : sc_bytes_b;
+    };
+    // MFMA of block (i, b): step of the K tile, and the scales of that K tile
+    auto multiply = [&](auto i_tag, auto b_tag, auto step_tag, auto first_tag, const vec8& fb, const vec8& fa, const int(&sc)[8]) __attribute__((always_inline)) {
+      constexpr int i = decltype(i_tag)::value, b = decltype(b_tag)::value, step = decltype(step_tag)::value;
+      constexpr int blk = 8 * i + b;
+      if constexpr (MX) {
+        const int s_a = sc[2 * (i >> 2) + (i & 1)], s_b = sc[4 + 2 * (b >> 2) + (b & 1)];
+        const i32x4 xb = __builtin_bit_cast(i32x4, fb), xa = __builtin_bit_cast(i32x4, fa);
+        if constexpr (decltype(first_tag)::value) W4MxMfma::first<blk, step, (b >> 1) & 1, (i >> 1) & 1>(xb, xa, s_b, s_a);
+        else W4MxMfma::fma<blk, step, (b >> 1) & 1, (i >> 1) & 1>(xb, xa, s_b, s_a);
+      } else {
+        if constexpr (decltype(first_tag)::value) Mfma::template first<blk>(fb, fa);
+        else Mfma::template fma<blk>(fb, fa);
+      }
+    };
 
     // ---- output --------------------------------------------------------------------------------
     // acc[i][b][e]: row 128 wm + 16 i + r, column 128 wn + 32 (b / 2) + 8 g + 4 (b % 2) + e of the tile.
@@ -426,11 +512,11 @@ struct GemmW4 {
         // row blocks in turn, the B fragments forwards and backwards alternately: consecutive MFMAs always
         // share one operand (fewer input toggles; this part is power limited)
         constexpr int i = m >> 3, b = (i & 1) ? 7 - (m & 7) : (m & 7);
-        constexpr int blk = 8 * i + b;
+        using Block = std::integral_constant<int, i>;
+        using Column = std::integral_constant<int, b>;
         if constexpr (half == 0 && LN && FIRST) asm volatile("s_nop 0");
-        else if constexpr (half == 0) Mfma::template fma<blk>(fb1[b], fa1[i]);
-        else if constexpr (FIRST) Mfma::template first<blk>(fb0[b], fa0[i]);
-        else Mfma::template fma<blk>(fb0[b], fa0[i]);
+        else if constexpr (half == 0) multiply(Block{}, Column{}, std::integral_constant<int, 1>{}, std::false_type{}, fb1[b], fa1[i], cur);
+        else multiply(Block{}, Column{}, std::integral_constant<int, 0>{}, first_tag, fb0[b], fa0[i], nxt);
         // the gap
         if constexpr (gap == G0 - 1) {
           // Two MFMAs of the previous K tile are in the matrix core's queue while the wavefronts meet.
@@ -451,8 +537,9 @@ struct GemmW4 {
         }
         if constexpr (ld >= 0) {
           using Fresh = std::bool_constant<FIRST && ld == 0>;
-          if constexpr (half == 0) load_tile_part(ld_b, voff_b[ld], Fresh{});
-          else load_tile_part(ld_a, voff_a[ld], Fresh{});
+          using Load = std::integral_constant<int, ld>;
+          if constexpr (half == 0) load_tile_part(ld_b, voff_b[ld], Load{}, Fresh{});
+          else load_tile_part(ld_a, voff_a[ld], Load{}, Fresh{});
         } else if constexpr (rd >= 0 && rd < B_READS) {
           if constexpr (B_KMAJOR) {
             const i32x2 v = read_b_transposed(sb, half, rd);  // K elements 0..3 (even read) or 4..7 of the lane's 8
@@ -477,19 +564,29 @@ struct GemmW4 {
         if constexpr (half == 1 && m == LAST_READ + 1) rd_a = rd_a + SLOT == B_REGION ? 0 : rd_a + SLOT;
         if constexpr (half == 1 && m == LAST_READ + 2) rd_b = rd_b + SLOT == LDS_BYTES ? B_REGION : rd_b + SLOT;
         if constexpr (half == 1 && m > LAST_A && m <= LAST_A + 3) advance(ld_a, wrap_a, next_a, 0, B_REGION, a_step, a_end, m - LAST_A - 1);
+        // the scales of this K tile, loaded during the one before, are made ready; those of the next one are asked for
+        if constexpr (MX && gap >= 32 && gap < 48 && (gap & 3) == 0) turn_scales(std::integral_constant<int, (gap - 32) / 4>{});
+        if constexpr (MX && gap >= 48 && gap < 56 && (gap & 1) == 0) load_scales(std::integral_constant<int, (gap - 48) / 2>{});
+        if constexpr (MX && gap == 57) advance_scales();
         if constexpr (FIRST && !LN && gap >= 10 && gap < 10 + 8 * FM && ((gap - 10) & 1) == 0) {
           // pair q of row block i goes into gap 10 + 8 i + 2 q
           store_pair(std::integral_constant<int, (gap - 10) / 8>{}, std::integral_constant<int, ((gap - 10) / 2) % 4>{}, std::false_type{});
         }
         __builtin_amdgcn_sched_barrier(0);
       });
+      if constexpr (MX) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cur[e] = nxt[e];
+        // (a matrix instruction must not follow at once on one that writes its operand; the compiler does not see the ones here)
+        asm volatile("s_nop 1" : "+v"(cur[0]), "+v"(cur[1]), "+v"(cur[2]), "+v"(cur[3]), "+v"(cur[4]), "+v"(cur[5]), "+v"(cur[6]), "+v"(cur[7]));
+      }
     };
 
     auto load_whole_tile = [&](const Stream& st, const unsigned(&voff)[LPT]) __attribute__((always_inline)) {
       w4_static_for<0, LPT>([&](auto i_tag) __attribute__((always_inline)) {
         set_load_target(st, i_tag);
-        asm volatile("s_nop 0");  // the wait state between the write of M0 and its use
-        load_tile_part(st, voff[decltype(i_tag)::value], std::bool_constant<decltype(i_tag)::value == 0>{});
+        if constexpr (!MX) asm volatile("s_nop 0");  // the wait state between the write of M0 and its use
+        load_tile_part(st, voff[decltype(i_tag)::value], i_tag, std::bool_constant<decltype(i_tag)::value == 0>{});
       });
     };
     // Prologue: A and B of K tile 0, A of K tile 1 (oldest first: the first wait is about tile 0).
@@ -509,7 +606,8 @@ struct GemmW4 {
     auto drain = [&]() __attribute__((always_inline)) {
       w4_static_for<0, 64>([&](auto m_tag) __attribute__((always_inline)) {
         constexpr int m = decltype(m_tag)::value;
-        Mfma::template fma<m>(fb1[m & 7], fa1[m >> 3]);
+        multiply(std::integral_constant<int, (m >> 3)>{}, std::integral_constant<int, (m & 7)>{}, std::integral_constant<int, 1>{}, std::false_type{}, fb1[m & 7],
+                 fa1[m >> 3], cur);
       });
       asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     };
@@ -549,6 +647,12 @@ struct GemmW4 {
       }
     } else if (g_total > 0) {
       TileCoord tc_cur = tile_coord(0);
+      if constexpr (MX) {  // the scales of K tile 0, in front of the fills; the stream moves on to K tile 1
+        next_scales(0, tc_cur);
+        sc_a = next_sc_a, sc_b = next_sc_b, sc_bytes_a = next_sc_bytes_a, sc_bytes_b = next_sc_bytes_b;
+        w4_static_for<0, 4>([&](auto n_tag) __attribute__((always_inline)) { load_scales(n_tag); });
+        advance_scales();  // (n_k >= 3)
+      }
       prologue(rows_of_a(0, tc_cur), rows_of_b(0, tc_cur));
       for (int j = 0; j < my_tiles; ++j) {
         // The streams move on to tile j + 1 while tile j is multiplied: A in its last but one K tile,
@@ -557,6 +661,7 @@ struct GemmW4 {
         tc_cur = tile_coord(j + 1 < my_tiles ? j + 1 : j);
         next_a = rows_of_a(j + 1, tc_cur);
         next_b = rows_of_b(j + 1, tc_cur);
+        if constexpr (MX) next_scales(j + 1, tc_cur);
         k_tile(std::true_type{});
         out = out_tile_of(j, tc_j);  // from here on the accumulators belong to tile j
         for (int h = 1; h < n_k; ++h) k_tile(std::false_type{});
@@ -867,6 +972,12 @@ struct GemmW4 {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 };
+
+template <typename T, int STORE>
+__global__ void __launch_bounds__(256) gemm_mx_w4_kernel(const MxW4Params p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  GemmW4<T, STORE, false, 4, 8, 2, false, true>::run(p, smem);
+}
 
 template <typename T, int STORE = kStoreThrough, bool LN = false, int SB = 4, int SA = 8, int G0 = 2, bool B_KMAJOR = false>
 __global__ void __launch_bounds__(256) gemmrc_w4_kernel(const GemmParams p) {

@@ -40,6 +40,31 @@ struct MxParams {
   TileDivs divs;
 };
 
+// Where chunk c of a row's 8 lies in LDS before the row's XOR: lane group g reads place 4 step + g, as of 16-bit elements, for
+// which that XOR is made (chunks 2 g + step in their own places: a read's groups of lanes meet in the same banks, 8192^3
+// CONFLICTS us).  A fill has each lane fetch the chunk that belongs where it writes, from the same line.
+BEAM_HD int mx_place_of(int chunk) { return (chunk & 1) << 2 | chunk >> 1; }
+BEAM_HD int mx_chunk_at(int place) { return (place & 3) << 1 | place >> 2; }
+
+// For the kernel of gemm_w4.h: elements and K in units of 16 bits (4 columns).
+struct MxW4Params : GemmParams {
+  const uint8_t* sa;
+  const uint8_t* sb;
+};
+
+// The scales of four blocks of 16 rows, from 8 bytes a lane (those of row r of block g in lane (r, g)) to two registers of what a
+// lane needs of each block, 16 bits (chunks 2 g and 2 g + 1 of row r): blocks 0 and 2 in the first, 1 and 3 in the second.
+// Lane group j holds the four 16-bit words 0 .. 3 of its row of block j and needs word g of all four.  v_permlane32_swap makes
+// (words 0, 1 of blocks j and j + 2) in groups 0 and 1, (words 2, 3) in groups 2 and 3; their low words, and their high ones, go
+// into a register each; v_permlane16_swap changes the high ones of the even groups for the low ones of the odd groups.
+__device__ __forceinline__ void mx_turn(i32x2 rows, int* even, int* odd) {
+  const auto x = __builtin_amdgcn_permlane32_swap((unsigned)rows[0], (unsigned)rows[1], false, false);
+  const unsigned lo = __builtin_amdgcn_perm(x[1], x[0], 0x05040100u), hi = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
+  const auto y = __builtin_amdgcn_permlane16_swap(lo, hi, false, false);
+  *even = (int)y[0];
+  *odd = (int)y[1];
+}
+
 // acc += a x b for chunk step STEP, operand registers PA, PB of the pairs that share a scale register (0: low half, 1: high).
 // The first operand's rows become the columns of C, as everywhere here.
 template <int STEP, int PB, int PA>
@@ -107,6 +132,8 @@ template <typename T>
 hipError_t launch_gemm_mx(int block_m, int block_n, const MxParams& p, hipStream_t stream);
 template <> hipError_t launch_gemm_mx<_Float16>(int, int, const MxParams&, hipStream_t);
 template <> hipError_t launch_gemm_mx<__bf16>(int, int, const MxParams&, hipStream_t);
+// The kernel of gemm_w4.h (256 x 256 tiles, a workgroup per CU walks them): K % 256 == 0, K >= 768, N % 8 == 0, C on 16 bytes.
+hipError_t launch_gemm_mx_w4(const MxW4Params& p, int dtype, dim3 grid, hipStream_t stream);
 template <typename T>
 hipError_t launch_gemm_mx_kwave(int rows, int cols, bool a16, const MxParams& p, hipStream_t stream);
 template <> hipError_t launch_gemm_mx_kwave<_Float16>(int, int, bool, const MxParams&, hipStream_t);

@@ -69,7 +69,13 @@ size_t beam_dbg_ln_plan_bytes(int M, int N, int K, const beam_tile_cfg* cfg, int
  * 3 beam_gemmrc_ln's one-kernel form.  row_starts, of every row of A (and of B as [N][K]): 0 at an element, 1 on 16 bytes
  * (K % 8 == 0), 2 on 128 (K % 64 == 0).  Before a device has been probed, of one with 256 CUs. */
 int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, int* cols, int* waves, int* whole_lines);
-/* What beam_gemmrc_mxfp4 runs an M x N x K problem on: a tile of rows x cols, kwave 1 if its K tiles are dealt out to the wavefronts. */
+/* Measurement only: the tile that MXFP4 products, and gated layers, run on from now on, named as beam_dbg_mx_tile and
+ * beam_dbg_gated_tile name it, whether it suits the problem or not; rows = 0: the library's choice again.  A tile that is not
+ * compiled makes the calls fail. */
+int beam_dbg_set_mx_tile(int rows, int cols, int kwave);
+int beam_dbg_set_gated_tile(int rows, int cols, int kind);
+/* What beam_gemmrc_mxfp4 runs an M x N x K problem on: a tile of rows x cols, *kwave 1 if its K tiles are dealt out to the wavefronts,
+ * 2 if a workgroup on each CU walks the tiles (C on 16 bytes). */
 int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave);
 /* What beam_gemmrc_gated runs an M x N x K problem on (K from 8 on): rows x cols rows of A and B, kind 0 tiles of gemm_kernel.h,
  * 2 the deep ones, 3 those that fill by whole lines, 4 tiles of gemm_kwave.h, 5 those that fill by whole lines.  row_starts as in
