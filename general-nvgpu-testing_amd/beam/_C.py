@@ -105,7 +105,7 @@ def _load() -> ctypes.CDLL:
     L.beam_silu.argtypes = [vp, vp, ctypes.c_longlong, i, vp]
     L.beam_matmul_nn.argtypes = [vp, vp, vp, i, i, i, i, cfgp, vp]
     L.beam_gemmrc_gated.argtypes = [vp, vp, vp, vp, i, i, i, i, vp]
-    L.beam_gemmrc_gated_backward_workspace_bytes.argtypes = [i, i, i, i]
+    L.beam_gemmrc_gated_backward_workspace_bytes.argtypes = [i, i, i, i, i]
     L.beam_gemmrc_gated_backward_workspace_bytes.restype = sz
     L.beam_gemmrc_gated_backward.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
     L.beam_mxfp4_scale_bytes.argtypes = [i, i]
@@ -143,6 +143,7 @@ def _load() -> ctypes.CDLL:
     L.beam_dbg_assume_compute_units.argtypes = [i]
     L.beam_dbg_small_tile.argtypes = [i, i, i, i, i] + [ctypes.POINTER(i)] * 4
     L.beam_dbg_set_mx_tile.argtypes = L.beam_dbg_set_gated_tile.argtypes = [i, i, i]
+    L.beam_dbg_set_nn_split.argtypes = [i, i]
     L.beam_dbg_mx_tile.argtypes = [i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_gated_tile.argtypes = [i, i, i, i] + [ctypes.POINTER(i)] * 3
     L.beam_dbg_nn_off_lines_tile.argtypes = [i, i, i, cfgp, cfgp, ctypes.POINTER(i)]
@@ -661,7 +662,7 @@ def gemmrc_gated_backward(dh, gu, a, b, da=None, db=None) -> None:
         pdh, pgu = _matrix(dh, "dh", M, N2 // 2, d)[0], _matrix(gu, "gu", M, N2, d)[0]
         pda = _matrix(da, "da", M, K, d)[0] if da is not None else None
         pdb = _matrix(db, "db", N2, K, d)[0] if db is not None else None
-        need = lib.beam_gemmrc_gated_backward_workspace_bytes(M, N2 // 2, da is not None, db is not None)
+        need = lib.beam_gemmrc_gated_backward_workspace_bytes(M, N2 // 2, K, da is not None, db is not None)
         ws, keep = _call_workspace(a, need)
         _check(lib.beam_gemmrc_gated_backward(pdh, pgu, pa, pb, pda, pdb, M, N2 // 2, K, d, ws, need, _stream_of(a)))
         del keep

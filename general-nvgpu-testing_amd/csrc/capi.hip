@@ -1054,6 +1054,47 @@ GatedTile gated_tile(int M, int N, int K, RowStarts rows, int cus) {
   return GatedTile{c.block_m, c.block_n, c.pipeline == 2 && c.block_m * c.block_n == 128 * 128 ? kGatedDeep : kGatedShallow};
 }
 
+// How a product of the backward pass, C [M][N] with B as [K][N], is cut into K slices; fewer than two: matmul_nn as it is.  What
+// slices save, a long sum on few CUs, has to pay for their partial sums and for a launch that adds them, 4 us and more: sums of
+// 4096 and more, on up to a third of the CUs.  us of the whole pass, without -> with (tokens x N x K): 16 x 11008 x 4096 139 -> 101,
+// 128 x 11008 x 4096 162 -> 116, 300 x 4096 x 1024 50 -> 36, 1024 x 2816 x 1024 58.7 -> 53.5; half the CUs 1001 x 2001 x 2000 67.7,
+// 66.1; shorter sums 512 x 1024 x 512 17.0, 29.7; 1024 x 1024 x 1024 26.5, 31.4.
+struct NnSplit {
+  int block_m, slices;
+};
+std::atomic<int> g_nn_split_rows{-1}, g_nn_split_slices{0};  // beam_dbg_set_nn_split
+NnSplit nn_split(int M, int N, int K, int cus) {
+  if (const int rows = g_nn_split_rows.load(std::memory_order_relaxed); rows >= 0) return NnSplit{rows, g_nn_split_slices.load(std::memory_order_relaxed)};
+  const int rows = M <= 64 ? 64 : 128;
+  const long tiles = (long)((M + rows - 1) / rows) * ((N + 127) / 128);
+  return NnSplit{rows, K >= 4096 && tiles * 3 <= cus ? auto_slices(tiles, K, cus) : 1};
+}
+int nn_slices(const NnSplit& s, int K) {  // no empty ones
+  const int ktiles = (K + kBK - 1) / kBK;
+  if (s.slices < 2 || ktiles < 2) return 1;
+  const int each = (ktiles + (s.slices < ktiles ? s.slices : ktiles) - 1) / (s.slices < ktiles ? s.slices : ktiles);
+  return (ktiles + each - 1) / each;
+}
+size_t nn_split_bytes(int M, int N, int K, int cus) {
+  const int s = nn_slices(nn_split(M, N, K, cus), K);
+  return s < 2 ? 0 : align_up((size_t)s * M * N * sizeof(float), 256);
+}
+int run_nn_split(const void* A, const void* B, void* C, int M, int N, int K, int b_rows, int dtype, void* ws, hipStream_t st) {
+  const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
+  const NnSplit split = nn_split(M, N, K, cus);
+  const int s = nn_slices(split, K);
+  if (s < 2) return matmul_nn(A, B, C, M, N, K, b_rows, dtype, nullptr, st);
+  const beam_tile_cfg c = {split.block_m, 128, 0, 0, 0, default_group_m(split.block_m, 128)};
+  GemmParams p = base_params(A, B, M, N, K, c);
+  p.ws = (float*)ws;
+  p.b_rows = b_rows;
+  p.splits = s;
+  p.k_slice = ((K + kBK - 1) / kBK + s - 1) / s * kBK;
+  BEAM_HIP(launch_partial_kmajor(split.block_m, p, dtype, st));
+  BEAM_HIP(launch_splitk_reduce(p.ws, C, (size_t)M * N, s, dtype, nullptr, st));
+  return BEAM_OK;
+}
+
 // A [M][K] and the layer's 2 N rows of B: what every entry refuses.
 int check_gated(const void* A, const void* B, const void* H, int M, int N, int K, int dtype, bool* generic) {
   if (N > INT32_MAX / 4) return fail(BEAM_ERR_UNSUPPORTED, "N=%d too large", N);
@@ -1108,9 +1149,21 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
 // us, rows as long as they are -> whole lines: 1001 x 2001 x 2000 bf16, dA 31.3 -> GATED_DA, dB 27.0 -> GATED_DB.
 static int gated_line(int n) { return (n + kBK - 1) / kBK * kBK; }
 
-size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int want_dA, int want_dB) {
+static size_t gated_operand_bytes(int M, int N, int want_dA, int want_dB) {
   if (M <= 0 || N <= 0 || N > INT32_MAX / 4) return 0;
   return (want_dA ? align_up((size_t)M * gated_line(2 * N) * 2, 256) : 0) + (want_dB ? align_up((size_t)2 * N * gated_line(M) * 2, 256) : 0);
+}
+
+// Whether the products take rows of whole lines; then they may also be cut into slices.
+static bool gated_lines(int M, int N, int K) { return K % 8 == 0 && K <= (1 << 23) && gated_line(2 * N) <= kMaxK && gated_line(M) <= kMaxK; }
+
+size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int K, int want_dA, int want_dB) {
+  const size_t operands = gated_operand_bytes(M, N, want_dA, want_dB);
+  if (operands == 0 || K <= 0 || !gated_lines(M, N, K)) return operands;
+  (void)beam_init();  // the number of slices depends on the device; a call on a host without one is refused there
+  const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
+  const size_t a = want_dA ? nn_split_bytes(M, K, gated_line(2 * N), cus) : 0, b = want_dB ? nn_split_bytes(2 * N, K, gated_line(M), cus) : 0;
+  return operands + (a > b ? a : b);  // one after the other
 }
 
 int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
@@ -1124,18 +1177,22 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
   if ((size_t)((M + 63) / 64) * ((N + 63) / 64) > INT32_MAX) return fail(BEAM_ERR_UNSUPPORTED, "M=%d x N=%d too large", M, N);
   if (dB && (2 * N + 63) / 64 > 65535) return fail(BEAM_ERR_UNSUPPORTED, "N=%d too large for dB", N);
   if (M > 0 && N > 0 && (!dH || !GU)) return fail(BEAM_ERR_INVALID, "null input pointer");
-  const size_t need = beam_gemmrc_gated_backward_workspace_bytes(M, N, dA != nullptr, dB != nullptr);
+  const size_t need = beam_gemmrc_gated_backward_workspace_bytes(M, N, K, dA != nullptr, dB != nullptr);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255) != 0))
     return fail(BEAM_ERR_WORKSPACE, "workspace of %zu bytes on 256 needed, %zu given", need, ws ? ws_bytes : (size_t)0);
   if ((rc = beam_init())) return rc;
   char* const d = (char*)ws;
   char* const dt = d + (dA ? align_up((size_t)M * gated_line(2 * N) * 2, 256) : 0);
-  const bool lines = K % 8 == 0 && K <= (1 << 23) && gated_line(2 * N) <= kMaxK && gated_line(M) <= kMaxK;
+  const bool lines = gated_lines(M, N, K);
+  char* const sums = d + gated_operand_bytes(M, N, dA != nullptr, dB != nullptr);
   const int cols_d = lines ? gated_line(2 * N) : 2 * N, cols_dt = lines ? gated_line(M) : M;
   if (M > 0 && N > 0) BEAM_HIP(launch_gated_gradients(dH, GU, dA ? d : nullptr, dB ? dt : nullptr, M, N, cols_d, cols_dt, dtype, (hipStream_t)stream));
-  if (dA && (rc = matmul_nn(d, B, dA, M, K, cols_d, 2 * N, dtype, nullptr, stream))) return rc;
-  if (dB && (rc = matmul_nn(dt, A, dB, 2 * N, K, cols_dt, M, dtype, nullptr, stream))) return rc;
-  return BEAM_OK;
+  if (!lines || M == 0 || N == 0) {
+    if (dA && (rc = matmul_nn(d, B, dA, M, K, cols_d, 2 * N, dtype, nullptr, stream))) return rc;
+    return dB ? matmul_nn(dt, A, dB, 2 * N, K, cols_dt, M, dtype, nullptr, stream) : BEAM_OK;
+  }
+  if (dA && (rc = run_nn_split(d, B, dA, M, K, cols_d, 2 * N, dtype, sums, (hipStream_t)stream))) return rc;
+  return dB ? run_nn_split(dt, A, dB, 2 * N, K, cols_dt, M, dtype, sums, (hipStream_t)stream) : BEAM_OK;
 }
 
 // ---- MXFP4 ------------------------------------------------------------------------------------
@@ -2097,6 +2154,12 @@ int beam_dbg_set_mx_tile(int rows, int cols, int kwave) {
   g_mx_cols.store(cols);
   g_mx_kwave.store(kwave);
   g_mx_rows.store(rows);
+  return BEAM_OK;
+}
+
+int beam_dbg_set_nn_split(int rows, int slices) {
+  g_nn_split_slices.store(slices);
+  g_nn_split_rows.store(rows);
   return BEAM_OK;
 }
 

@@ -55,6 +55,9 @@ hipError_t launch_gated_kwave(const KwPlan& plan, const KwGatedParams& p, hipStr
 template <> hipError_t launch_gated_kwave<_Float16>(const KwPlan&, const KwGatedParams&, hipStream_t);
 template <> hipError_t launch_gated_kwave<__bf16>(const KwPlan&, const KwGatedParams&, hipStream_t);
 
+// p.ws [splits][M][N] fp32: the sums of K slices of A . B with B as [K][N], in tiles of block_m x 128, block_m 64 or 128.
+hipError_t launch_partial_kmajor(int block_m, const GemmParams& p, int dtype, hipStream_t stream);
+
 // Any sizes, element by element (what the tiled kernels refuse: K below 8 or beyond a descriptor).
 hipError_t launch_gated_plain(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, hipStream_t stream);
 

@@ -48,32 +48,40 @@ __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restric
   const int m0 = tm * R, n0 = tn * C;
   const int c = threadIdx.x & 7, rp = threadIdx.x >> 3;
   const int n = n0 + 8 * c;
+  // All loads in front of any arithmetic.  Behind the last row the last one is read again, behind the last column, where 8 do not
+  // fit, single elements and the last one again: what is made of those is not stored, but for zeros behind row M in DT.
+  vec8 g[2], u[2], d[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const size_t m = m0 + 2 * rp + h < M ? m0 + 2 * rp + h : M - 1;
+    const T* const gu = GU + m * 2 * N;
+    const T* const dh = dH + m * N;
+    if (n0 + C <= N) {  // (uniform)
+      g[h] = *(const vec8_at_element*)(gu + n);
+      u[h] = *(const vec8_at_element*)(gu + N + n);
+      d[h] = *(const vec8_at_element*)(dh + n);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int col = n + e < N ? n + e : N - 1;
+        g[h][e] = gu[col];
+        u[h][e] = gu[N + col];
+        d[h][e] = dh[col];
+      }
+    }
+  }
   vec8 dg[2], du[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int m = m0 + 2 * rp + h;
-    vec8 g, u, d;
-    const size_t at = (size_t)m * N + n, at_g = (size_t)m * 2 * N + n;
-    if (m < M && n + 7 < N) {
-      g = *(const vec8_at_element*)(GU + at_g);
-      u = *(const vec8_at_element*)(GU + at_g + N);
-      d = *(const vec8_at_element*)(dH + at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool there = m < M && n + e < N;
-        g[e] = there ? GU[at_g + e] : (T)0.0f;
-        u[e] = there ? GU[at_g + N + e] : (T)0.0f;
-        d[e] = there ? dH[at + e] : (T)0.0f;
-      }
-    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float gf = (float)g[e], df = (float)d[e];
+      const float gf = (float)g[h][e], df = (float)d[h][e];
       const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gf * -1.4426950408889634f));
-      dg[h][e] = (T)(df * (float)u[e] * (s * (1.0f + gf * (1.0f - s))));
+      dg[h][e] = (T)(df * (float)u[h][e] * (s * (1.0f + gf * (1.0f - s))));
       du[h][e] = (T)(df * (gf * s));
     }
+    if (m >= M) dg[h] = du[h] = vec8{};  // (whatever the nearest row holds)
     if (D && m < M) {
       T* const row = D + (size_t)m * cols_d + n;
       if (n + 7 < N) {

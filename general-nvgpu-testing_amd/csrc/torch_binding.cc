@@ -238,7 +238,7 @@ PyObject* gemmrc_gated_backward(PyObject*, PyObject* const* args, Py_ssize_t n) 
     const bool want_a = args[4] != Py_None, want_b = args[5] != Py_None;
     if ((want_a && !is_matrix(args[4], dev, a.dtype, M, K, &da)) || (want_b && !is_matrix(args[5], dev, a.dtype, N2, K, &db))) return kNotHandled;
     void* const stream = c10::hip::getCurrentHIPStream().stream();
-    const size_t bytes = beam_gemmrc_gated_backward_workspace_bytes((int)M, (int)(N2 / 2), want_a, want_b);
+    const size_t bytes = beam_gemmrc_gated_backward_workspace_bytes((int)M, (int)(N2 / 2), (int)K, want_a, want_b);
     const c10::DataPtr ws = call_workspace(bytes);
     int rc;
     Py_BEGIN_ALLOW_THREADS;

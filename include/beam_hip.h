@@ -271,10 +271,11 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
 
 /* The gradients of that layer: with s = 1 / (1 + exp(-G)), D = [dH * U * s * (1 + G * (1 - s)), dH * G * s] ([M][2N], rounded to
  * the dtype for the products that follow), dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or
- * dB may be null: not asked for.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches; the workspace (256-byte
- * aligned, any contents) holds D and its transpose and belongs to the call until it has run: calls that overlap in time need one
+ * dB may be null: not asked for.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches, and one more for a
+ * product of so few outputs that its sums are cut into slices, which are added in their order; the workspace (256-byte
+ * aligned, any contents) holds D, its transpose and such sums, and belongs to the call until it has run: calls that overlap in time need one
  * each, and so does a captured graph that may run beside another. */
-size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int want_dA, int want_dB);
+size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int K, int want_dA, int want_dB);
 int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
                                int dtype, void* ws, size_t ws_bytes, void* stream);
 

@@ -74,6 +74,9 @@ int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, 
  * compiled makes the calls fail. */
 int beam_dbg_set_mx_tile(int rows, int cols, int kwave);
 int beam_dbg_set_gated_tile(int rows, int cols, int kind);
+/* ... and how the products of a gated layer's backward pass are cut into K slices, in tiles of rows (64, 128) x 128; slices = 1: not at
+ * all; rows = -1: the library's choice again. */
+int beam_dbg_set_nn_split(int rows, int slices);
 /* What beam_gemmrc_mxfp4 runs an M x N x K problem on: a tile of rows x cols, *kwave 1 if its K tiles are dealt out to the wavefronts,
  * 2 if a workgroup on each CU walks the tiles (C on 16 bytes). */
 int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave);

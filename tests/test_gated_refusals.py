@@ -29,9 +29,9 @@ def test_forward(beamc):
 
 def test_backward(beamc):
     f, need = beamc.lib.beam_gemmrc_gated_backward, beamc.lib.beam_gemmrc_gated_backward_workspace_bytes
-    n = need(100, 60, 1, 1)
-    assert n == need(100, 60, 1, 0) + need(100, 60, 0, 1) and min(need(100, 60, 1, 0), need(100, 60, 0, 1)) >= 100 * 120 * 2 and n % 256 == 0
-    assert need(0, 60, 1, 1) == need(100, 0, 1, 1) == need(100, 60, 0, 0) == 0
+    n = need(100, 60, 8, 1, 1)
+    assert n <= need(100, 60, 8, 1, 0) + need(100, 60, 8, 0, 1) and min(need(100, 60, 8, 1, 0), need(100, 60, 8, 0, 1)) >= 100 * 120 * 2 and n % 256 == 0
+    assert need(0, 60, 8, 1, 1) == need(100, 0, 8, 1, 1) == need(100, 60, 8, 0, 0) == 0
     good = [P, P, P, P, P, P, 100, 60, 8, F16, P, n, None]
 
     def but(**kw):

@@ -213,7 +213,7 @@ def run_backward(beamc, dh, gu, a, b, dtype, offsets=(0,) * 6, want=(True, True)
     N = b.shape[0] // 2
     ins = [Guarded(beamc, x, o, dtype) for x, o in zip((dh, gu, a, b), offsets)]
     da, db = Guarded(beamc, (M, K), offsets[4], dtype), Guarded(beamc, (2 * N, K), offsets[5], dtype)
-    need = beamc.lib.beam_gemmrc_gated_backward_workspace_bytes(M, N, *want)
+    need = beamc.lib.beam_gemmrc_gated_backward_workspace_bytes(M, N, K, *want)
     ws = beamc.DeviceArray((need + 256,), itemsize=1)
     ws.fill_bytes(0xFF)
     beamc._check(beamc.lib.beam_gemmrc_gated_backward(*[t.ptr for t in ins], da.ptr if want[0] else None, db.ptr if want[1] else None,
@@ -332,7 +332,7 @@ def test_graph_of_a_training_step(gpu, beamc):
     L, chk = beamc.lib, beamc._check
     M, N, K = 203, 310, 264
     a, b, dh = (beamc.DeviceArray(s, BF16) for s in ((M, K), (2 * N, K), (M, N)))
-    need = L.beam_gemmrc_gated_backward_workspace_bytes(M, N, 1, 1)
+    need = L.beam_gemmrc_gated_backward_workspace_bytes(M, N, K, 1, 1)
 
     def results():
         return [beamc.DeviceArray(s, BF16) for s in ((M, N), (M, 2 * N), (M, K), (2 * N, K))] + [beamc.DeviceArray((need,), itemsize=1)]
@@ -364,3 +364,48 @@ def test_graph_of_a_training_step(gpu, beamc):
             assert (x.to_numpy() == y.to_numpy()).all(), replay
     chk(L.beam_graph_destroy(graph))
     chk(L.beam_stream_destroy(stream))
+
+
+def test_backward_of_infinities_in_the_last_row(gpu, beamc, oracle):
+    """The last row's gradients are not finite: they reach its row of da and all of db's rows that they belong to, and nothing
+    comes from behind the last row, which is a whole line of the workspace away."""
+    M, N, K = 70, 40, 64
+    dh, gu, a, b = backward_inputs(beamc, M, N, K, F16)
+    clean = run_backward(beamc, dh, gu, a, b, F16)
+    gu2 = gu.copy()
+    gu2[M - 1, N + 5] = 0x7C00  # u of column 5 is infinite: dg of column 5 is, in the last row
+    da, db = run_backward(beamc, dh, gu2, a, b, F16)
+    bad = ~np.isfinite(oracle.to_f32(da, F16))
+    assert bad[M - 1].all() and not bad[:M - 1].any() and (da[:M - 1] == clean[0][:M - 1]).all()
+    bad = ~np.isfinite(oracle.to_f32(db, F16))
+    assert bad[5].all() and bad.sum() == K
+    keep = np.arange(2 * N) != 5
+    assert (db[keep] == clean[1][keep]).all()
+
+
+@pytest.mark.parametrize("rows,slices", [(64, 2), (64, 7), (128, 3), (128, 16)])
+@pytest.mark.parametrize("M,N,K", [(1, 65, 8), (65, 63, 72), (200, 333, 136), (777, 256, 320), (1001, 501, 504)])
+def test_backward_in_slices(gpu, beamc, oracle, rows, slices, M, N, K):
+    """Sums cut into slices, whatever the problem: more than there are K tiles, and a last one that is short."""
+    beamc.lib.beam_dbg_set_nn_split(rows, slices)
+    try:
+        for dtype, offsets in ((F16, (0,) * 6), (BF16, (1, 3, 5, 7, 1, 3))):
+            dh, gu, a, b = backward_inputs(beamc, M, N, K, dtype)
+            da, db = run_backward(beamc, dh, gu, a, b, dtype, offsets)
+            D = gradients(oracle, dh, gu, dtype)
+            check_products(D, f64(oracle, b, dtype), f64(oracle, da, dtype), HALF_STEP[dtype], TINY[dtype], ("da", M, N, K, dtype))
+            check_products(D.T, f64(oracle, a, dtype), f64(oracle, db, dtype), HALF_STEP[dtype], TINY[dtype], ("db", M, N, K, dtype))
+    finally:
+        beamc.lib.beam_dbg_set_nn_split(-1, 0)
+
+
+def test_backward_of_a_few_tokens_through_a_wide_layer(gpu, beamc, oracle):
+    """What the library cuts into slices by itself; the same bits again."""
+    for M, N, K in ((3, 4100, 264), (130, 2200, 136)):
+        dh, gu, a, b = backward_inputs(beamc, M, N, K, BF16)
+        da, db = run_backward(beamc, dh, gu, a, b, BF16)
+        D = gradients(oracle, dh, gu, BF16)
+        check_products(D, f64(oracle, b, BF16), f64(oracle, da, BF16), HALF_STEP[BF16], TINY[BF16], ("da", M, N, K))
+        check_products(D.T, f64(oracle, a, BF16), f64(oracle, db, BF16), HALF_STEP[BF16], TINY[BF16], ("db", M, N, K))
+        again = run_backward(beamc, dh, gu, a, b, BF16)
+        assert (again[0] == da).all() and (again[1] == db).all()
