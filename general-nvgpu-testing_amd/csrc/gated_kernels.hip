@@ -29,6 +29,19 @@ __global__ void __launch_bounds__(256) gated_plain_kernel(const T* __restrict__ 
   }
 }
 
+// v >> bits, 0 <= bits < 128, of eight 16-bit values
+template <typename V8>
+__device__ __forceinline__ V8 shift_down(V8 v, int bits) {
+  typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+  const u64x2 w = __builtin_bit_cast(u64x2, v);
+  const int b = bits & 63;
+  const unsigned long long over = b ? w[1] << (64 - b) : 0;
+  u64x2 o;
+  o[0] = bits >= 64 ? w[1] >> b : w[0] >> b | over;
+  o[1] = bits >= 64 ? 0 : w[1] >> b;
+  return __builtin_bit_cast(V8, o);
+}
+
 // With s = 1 / (1 + exp(-g)):  dg = dh * u * s * (1 + g * (1 - s)),  du = dh * g * s, in fp32, each rounded once to 16 bits,
 // which the products that follow take as operands.
 //
@@ -48,25 +61,38 @@ __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restric
   const int m0 = tm * R, n0 = tn * C;
   const int c = threadIdx.x & 7, rp = threadIdx.x >> 3;
   const int n = n0 + 8 * c;
-  // All loads in front of any arithmetic.  Behind the last row the last one is read again, behind the last column, where 8 do not
-  // fit, single elements and the last one again: what is made of those is not stored, but for zeros behind row M in DT.
+  const bool through = (N | cols_d) % 64 == 0;
+  // All loads in front of any arithmetic.  Behind the last row the last one is read again; 8 columns that do not fit are the row's
+  // last 8, shifted down; what is made of columns that do not exist is not stored, and of rows only zeros, in DT.
   vec8 g[2], u[2], d[2];
+  if (N >= 8) {  // (uniform)
+    const int at = n < N - 8 ? n : N - 8;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const size_t m = m0 + 2 * rp + h < M ? m0 + 2 * rp + h : M - 1;
-    const T* const gu = GU + m * 2 * N;
-    const T* const dh = dH + m * N;
-    if (n0 + C <= N) {  // (uniform)
-      g[h] = *(const vec8_at_element*)(gu + n);
-      u[h] = *(const vec8_at_element*)(gu + N + n);
-      d[h] = *(const vec8_at_element*)(dh + n);
-    } else {
+    for (int h = 0; h < 2; ++h) {
+      const size_t m = m0 + 2 * rp + h < M ? m0 + 2 * rp + h : M - 1;
+      g[h] = *(const vec8_at_element*)(GU + m * 2 * N + at);
+      u[h] = *(const vec8_at_element*)(GU + m * 2 * N + N + at);
+      d[h] = *(const vec8_at_element*)(dH + m * N + at);
+    }
+    if (n0 + C > N) {  // (uniform)
+      const int bits = (n - at) < 8 ? 16 * (n - at) : 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        g[h] = shift_down(g[h], bits);
+        u[h] = shift_down(u[h], bits);
+        d[h] = shift_down(d[h], bits);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const size_t m = m0 + 2 * rp + h < M ? m0 + 2 * rp + h : M - 1;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int col = n + e < N ? n + e : N - 1;
-        g[h][e] = gu[col];
-        u[h][e] = gu[N + col];
-        d[h][e] = dh[col];
+        g[h][e] = GU[m * 2 * N + col];
+        u[h][e] = GU[m * 2 * N + N + col];
+        d[h][e] = dH[m * N + col];
       }
     }
   }
@@ -85,8 +111,13 @@ __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restric
     if (D && m < M) {
       T* const row = D + (size_t)m * cols_d + n;
       if (n + 7 < N) {
-        *(vec8_at_element*)row = dg[h];
-        *(vec8_at_element*)(row + N) = du[h];
+        if (through) {
+          store_16<kStoreThrough>(row, __builtin_bit_cast(i32x4, dg[h]));
+          store_16<kStoreThrough>(row + N, __builtin_bit_cast(i32x4, du[h]));
+        } else {
+          *(vec8_at_element*)row = dg[h];
+          *(vec8_at_element*)(row + N) = du[h];
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -122,7 +153,8 @@ __global__ void __launch_bounds__(256) gated_gradients_kernel(const T* __restric
     const vec8 v = *(const vec8*)(turned + up * C * R + col * R + ((chunk ^ (col >> 3)) << 3));
     T* const out = DT + ((size_t)up * N + n0 + col) * cols_dt + m;
     if (m + 7 < cols_dt) {  // (behind M these are zeros)
-      *(vec8_at_element*)out = v;
+      if (cols_dt % 64 == 0) store_16<kStoreThrough>(out, __builtin_bit_cast(i32x4, v));
+      else *(vec8_at_element*)out = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
