@@ -1022,18 +1022,20 @@ std::atomic<int> g_gated_rows{0}, g_gated_cols{0}, g_gated_kind{0};  // beam_dbg
 KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
   if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) {
     const int kind = g_gated_kind.load(std::memory_order_relaxed);
-    return kind < 4 ? KwPlan{0, 0, 0, false} : KwPlan{forced, g_gated_cols.load(std::memory_order_relaxed), 4, kind == 5};
+    const bool fits = K >= 8 && K <= kMaxK && (forced > 8 || M <= 8) && (kind == 4 || (kind == 5 && rows != kAnywhere && forced > 8));
+    return fits ? KwPlan{forced, g_gated_cols.load(std::memory_order_relaxed), 4, kind == 5} : KwPlan{0, 0, 0, false};
   }
-  static const struct { int rows, cols; } kTiles[] = {{8, 32}, {16, 32}, {32, 32}, {8, 64}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
+  static const struct { int rows, cols; } kTiles[] = {{8, 32}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
   const KwPlan none = {0, 0, 0, false};
   if (K < 8 || K > kMaxK) return none;
   for (const auto& t : kTiles) {
     if (t.rows == 8 && M > 8) continue;
     const long tiles = ((long)M + t.rows - 1) / t.rows * (((long)N + t.cols / 2 - 1) / (t.cols / 2));
-    // a handful of rows: B is read once whatever the number of tiles
-    const bool few = M <= 16 && t.rows >= M && t.cols == 64;
+    // A handful of rows: B is read once whatever the number of tiles, and the smaller ones have more of it in flight on a CU
+    // (11008 x 4096 bf16, 16 columns of C to a tile, 32: 1 row 32.0 us, 37.1, 5.6 TB/s; 16 rows 34.3, 40.7).
+    const bool few = M <= 16 && t.rows >= M && t.cols == 32;
     if (tiles > cus && !few) continue;
-    const bool shift = rows == kOnChunks && t.rows > 8 && !(M <= 16 && t.cols == 64) && (long)(K / kBK) * (t.rows + t.cols) >= 1200;
+    const bool shift = rows == kOnChunks && t.rows > 8 && (long)(K / kBK) * (t.rows + t.cols) >= 1200;
     if (t.rows * t.cols == 64 * 64 && (rows == kOnLines ? K >= 2048 : shift)) return none;
     return KwPlan{t.rows, t.cols, 4, shift};
   }
@@ -1041,8 +1043,13 @@ KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
 }
 
 // The tile of the gated kernel: what beam_gemmrc would take for the 2 N rows of B, as far as there is one like it.
-GatedTile gated_tile(int M, int N, int K, RowStarts rows, int cus) {
-  if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) return GatedTile{forced, g_gated_cols.load(std::memory_order_relaxed), g_gated_kind.load(std::memory_order_relaxed)};
+// walk_fits: the outputs are on 16 bytes.
+GatedTile gated_tile(int M, int N, int K, RowStarts rows, bool walk_fits, int cus) {
+  const bool walk = walk_fits && K % kBK == 0 && K >= kW4MinK && N % 8 == 0 && N <= (1 << 20) && (size_t)(N + 128) * K * 2 < ((size_t)1 << 31);
+  if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) {
+    const int kind = g_gated_kind.load(std::memory_order_relaxed);
+    if ((kind != kGatedWalk || walk) && (kind != kGatedLines || rows != kAnywhere)) return GatedTile{forced, g_gated_cols.load(std::memory_order_relaxed), kind};
+  }
   if (K % kBK != 0 && rows == kOnChunks) {
     const LineChoice t = off_lines_tile(M, 2 * N, K, cus);
     if (t.lines) return GatedTile{t.cfg.block_m == 128 && t.cfg.block_n == 64 ? 64 : t.cfg.block_m, 128, kGatedLines};
@@ -1050,8 +1057,14 @@ GatedTile gated_tile(int M, int N, int K, RowStarts rows, int cus) {
   beam_tile_cfg c;
   int s;
   (void)choose_default(M, 2 * N, K, -1, &c, &s);
+  // From a round of workgroups on, the walking kernel, as in beam_gemmrc (choose_default names it by its wavefronts).
+  if (c.block_m == 256 && c.block_n == 256 && c.wave_m == 128 && c.wave_n == 128 && walk) return GatedTile{256, 256, kGatedWalk};
   if (c.block_m * c.block_n <= 128 * 64) return GatedTile{64, 128, c.pipeline == 2 ? kGatedDeep : kGatedShallow};
-  return GatedTile{c.block_m, c.block_n, c.pipeline == 2 && c.block_m * c.block_n == 128 * 128 ? kGatedDeep : kGatedShallow};
+  // One 128 x 128 tile to a CU: its long ring, but for the shortest sums (512 x 4096 x 1024 16.8 -> 14.7 us, 1024 x 1024 x 1024 10.8 -> 9.6,
+  // 140 x 4480 x 448 7.8 -> 7.6; 603 x 2240 x 216 7.0, 7.4; 309 x 10816 x 128 5.9, 9.1).
+  const long tiles = (long)((M + 127) / 128) * ((N + 63) / 64);
+  if (c.block_m * c.block_n == 128 * 128 && (c.pipeline == 2 || (tiles <= cus && K >= 448))) return GatedTile{128, 128, kGatedDeep};
+  return GatedTile{c.block_m, c.block_n, kGatedShallow};
 }
 
 // How a product of the backward pass, C [M][N] with B as [K][N], is cut into K slices; fewer than two: matmul_nn as it is.  What
@@ -1133,13 +1146,19 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
     BEAM_HIP(dtype == BEAM_F16 ? launch_gated_kwave<_Float16>(kw, p, st) : launch_gated_kwave<__bf16>(kw, p, st));
     return BEAM_OK;
   }
-  const GatedTile t = gated_tile(M, N, K, rows, cus);
+  const GatedTile t = gated_tile(M, N, K, rows, (((uintptr_t)H | (uintptr_t)GU) & 15) == 0, cus);
   const beam_tile_cfg c = {t.block_m, t.block_n / 2, 0, 0, 0, default_group_m(t.block_m, t.block_n)};
   GemmParams p = base_params(A, B, M, N, K, c);
   p.C = H;
   p.gu = GU;
+  const long tiles = (long)p.tiles_m * p.tiles_n;
+  if (t.depth == kGatedWalk) {
+    p.c_store = store_kind(c, 4, true, H, M, N, K);
+    BEAM_HIP(launch_gated_w4(p, dtype, dim3((unsigned)(tiles < cus ? tiles : cus)), st));
+    return BEAM_OK;
+  }
   p.c_store = store_kind(c, 0, false, H, M, N, K);
-  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, 1);
+  const dim3 grid((unsigned)tiles, 1, 1);
   BEAM_HIP(dtype == BEAM_F16 ? launch_gated<_Float16>(t, p, grid, st) : launch_gated<__bf16>(t, p, grid, st));
   return BEAM_OK;
 }
@@ -1236,14 +1255,15 @@ struct MxPlan {
 };
 std::atomic<int> g_mx_rows{0}, g_mx_cols{0}, g_mx_kwave{0};  // beam_dbg_set_mx_tile
 MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
-  if (const int rows = g_mx_rows.load(std::memory_order_relaxed)) return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), g_mx_kwave.load(std::memory_order_relaxed)};
+  const bool w4_fits = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
+  if (const int rows = g_mx_rows.load(std::memory_order_relaxed); rows && (g_mx_kwave.load(std::memory_order_relaxed) != 2 || w4_fits))
+    return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), g_mx_kwave.load(std::memory_order_relaxed)};
   static const struct { int rows, cols; } kSmall[] = {{16, 16}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
   auto tiles = [&](int r, int c) { return ((long)M + r - 1) / r * (((long)N + c - 1) / c); };
   for (const auto& t : kSmall) {
     const bool few = M <= 16 && t.rows == 16 && t.cols == 64;
     if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, 1};
   }
-  const bool w4_fits = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
   if (tiles(256, 256) >= cus) return MxPlan{256, 256, w4_fits ? 2 : 0};
   if (tiles(256, 128) >= cus) return MxPlan{256, 128, 0};
   if (tiles(128, 128) >= cus) return MxPlan{128, 128, 0};
@@ -2185,7 +2205,7 @@ int beam_dbg_gated_tile(int M, int N, int K, int row_starts, int* rows, int* col
     *rows = kw.rows, *cols = kw.cols, *kind = kw.shift ? 5 : 4;
     return BEAM_OK;
   }
-  const GatedTile t = gated_tile(M, N, K, (RowStarts)row_starts, cus);
+  const GatedTile t = gated_tile(M, N, K, (RowStarts)row_starts, true, cus);
   *rows = t.block_m, *cols = t.block_n, *kind = t.depth;
   return BEAM_OK;
 }

@@ -12,7 +12,7 @@ namespace beam {
 
 
 // A workgroup tile of the gated kernel: block_n rows of B, half of them gate and half up rows, so block_n / 2 columns of C.
-enum GatedDepth : int { kGatedShallow = 0, kGatedDeep = 2, kGatedLines = 3 };
+enum GatedDepth : int { kGatedShallow = 0, kGatedWalk = 1, kGatedDeep = 2, kGatedLines = 3 };
 struct GatedTile {
   int block_m, block_n, depth;
 };
@@ -40,12 +40,14 @@ struct GatedTile {
   X(8, 32, 4)                        \
   X(16, 32, 4)                       \
   X(32, 32, 4)                       \
-  X(8, 64, 4)                        \
   X(16, 64, 4)                       \
   X(32, 64, 4)                       \
   X(64, 32, 4)                       \
   X(64, 64, 4)
 
+// kGatedWalk: the kernel of gemm_w4.h, 256 x 256 tiles that a workgroup on each CU walks.  K % 64 == 0, K >= kW4MinK, N % 8 == 0, C and
+// gu on 16 bytes, (N + 128) * K * 2 below 2^31, N at most 2^20.
+hipError_t launch_gated_w4(const GemmParams& p, int dtype, dim3 grid, hipStream_t stream);
 template <typename T>
 hipError_t launch_gated(const GatedTile& tile, const GemmParams& p, dim3 grid, hipStream_t stream);
 template <> hipError_t launch_gated<_Float16>(const GatedTile&, const GemmParams&, dim3, hipStream_t);

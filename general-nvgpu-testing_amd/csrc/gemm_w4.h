@@ -164,10 +164,17 @@ __host__ __device__ inline int w4_b_row(int b, int r) { return 32 * (b >> 1) + 4
 // tile, straight into registers (64 rows of 8 bytes each: MxScales' way of four blocks), asked for one K tile ahead behind the B
 // fills, exchanged between the lane groups while the K tile before is multiplied.  The fills are the compiler's builtins here: it
 // then knows that they are younger than the scales' loads and does not wait for all of them.
-template <typename T, int STORE = kStoreThrough, bool LN = false, int SB = 4, int SA = 8, int G0 = 2, bool B_KMAJOR = false, bool MX = false>
+// GATED: the gated layer (gemm_kernel.h: kEpiGated).  Of the blocks of a wavefront's tile the even ones are gate rows of B and the odd
+// ones up rows, dealt out so that a lane holds both factors of 8 consecutive columns in four blocks; a tile has 128 columns of C.
+// A B fill's 8 rows are then 4 gate and 4 up rows, N rows apart: one descriptor spans both (the host sees to N * K).  The
+// products are made and stored, like a plain tile's sums, while the next tile's first K tile is multiplied, two a gap; that K tile
+// takes as long as their exponentials and reciprocals, about three times its MFMAs.  With GU its factors are stored on the way.
+template <typename T, int STORE = kStoreThrough, bool LN = false, int SB = 4, int SA = 8, int G0 = 2, bool B_KMAJOR = false, bool MX = false, bool GATED = false>
 struct GemmW4 {
   static_assert(!(LN && B_KMAJOR), "the fused LayerNorm is built for B as [N][K]");
   static_assert(!(MX && (LN || B_KMAJOR)), "MXFP4 is built for the plain product");
+  static_assert(!(GATED && (LN || B_KMAJOR || MX)), "the gated layer is built for B as [2 N][K]");
+  static constexpr int CN = GATED ? 128 : 256;  // columns of C in a tile
   using Params = std::conditional_t<MX, MxW4Params, GemmParams>;
   using Traits = ElemTraits<T>;
   using vec8 = typename Traits::vec8;
@@ -253,6 +260,10 @@ struct GemmW4 {
         // 1 KiB = rows k, k + 1 of the [K][N] tile, k = 8 i + 2 w; lane l fills position l % 32 of row k + l / 32
         const int k = 8 * i + 2 * wave + (lane >> 5);
         voff_b[i] = ((unsigned)k * (unsigned)N + (unsigned)(((lane & 31) ^ w4_kmajor_swizzle(k)) << 3)) * 2u;
+      } else if constexpr (GATED) {
+        // row n = fill_row + 32 i of the tile of B: gate or up row (bit 2 of n) of column 32 (n / 64) + 8 (n / 8 % 4) + 4 (n / 32 % 2) + n % 4
+        const unsigned up = (fill_row >> 2) & 1, column = 32 * (i >> 1) + 4 * (i & 1) + 8 * ((fill_row >> 3) & 3) + (fill_row & 3);
+        voff_b[i] = (up * (unsigned)N + column) * (unsigned)K * 2u + (unsigned)(place_b << 4);
       } else {
         voff_b[i] = row_bytes + (unsigned)((MX ? mx_chunk_at(place_b) : place_b) << 4);
       }
@@ -269,8 +280,10 @@ struct GemmW4 {
     };
     auto rows_of_b = [&](int j, TileCoord tc) {
       if (j >= my_tiles) return make_rsrc(p.B, 0u);
-      const int col0 = tc.tn * BN;
-      const int rows = (N - col0) < BN ? (N - col0) : BN;
+      const int col0 = tc.tn * CN;
+      const int rows = (N - col0) < CN ? (N - col0) : CN;
+      // from the first gate row to the last up row; gate rows behind the last one are up rows, for columns that do not exist
+      if constexpr (GATED) return make_rsrc((const T*)p.B + (size_t)col0 * K, ((unsigned)N + (unsigned)rows) * (unsigned)K * 2u);
       // [K][N]: the tile's columns of all K rows (the range check counts the scalar offset, which holds the K
       // tile here, together with the per-lane one).  Columns past the tile's last one read the next row's data,
       // past the last row's end nothing: they only feed output columns that do not exist.
@@ -455,6 +468,22 @@ struct GemmW4 {
       return o;
     };
     OutTile out = out_tile_of(-1, TileCoord{0, 0});  // the tile whose accumulators are being stored
+    // GATED: the same of C's columns in groups of 8, voff[0] and voff[1], and of GU (its bytes: 0 without)
+    auto gated_out = [&](int j, TileCoord tc, void* to, int ld) {
+      OutTile o;
+      const int row0 = tc.tm * BM, col0 = tc.tn * CN;
+      const int rows = (M - row0) < BM ? (M - row0) : BM, cols = (N - col0) < CN ? (N - col0) : CN;
+      const bool none = j < 0 || j >= my_tiles || to == nullptr;
+      o.base = none ? (char*)p.C : (char*)((T*)to + ((size_t)row0 * ld + col0));
+      o.bytes = none ? 0 : ((rows - 1) * ld + cols) * 2;
+#pragma unroll
+      for (int q = 0; q < FN / 2; ++q) {
+        const int col = wn * 64 + 32 * q + 8 * g;
+        o.voff[q] = q < 2 && col < cols ? ((unsigned)(wm * 128 + r) * (unsigned)ld + (unsigned)col) * 2u : kOobOffset;
+      }
+      return o;
+    };
+    OutTile out_gate = out, out_up = out;
     // LAST: the stores after the workgroup's last K loop.  Nothing hides them, and a kernel ends only when its
     // dirty lines have left the L2: those go through it to memory at once (device-scope stores; 4096^3, one tile
     // per workgroup: 98.9 -> 96.5 us, fused LayerNorm 105.7 -> 103.7 us).  The stores of earlier tiles lie under
@@ -482,6 +511,40 @@ struct GemmW4 {
       const int left = out.bytes - skip;
       const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(out.base + skip, left > 0 ? (unsigned)left : 0u);
       __builtin_amdgcn_raw_buffer_store_b128(w, rsrc, (int)out.voff[q], 0, AUX);
+    };
+
+    auto gated_store = [&](const OutTile& to, auto i_tag, auto q_tag, int ld, i32x4 w, auto last_tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(i_tag)::value, q = decltype(q_tag)::value;
+      constexpr int AUX = STORE == kStoreStreaming ? 2 : (decltype(last_tag)::value && STORE == kStoreThrough ? kAuxDeviceScope : 0);
+      const int skip = i * 16 * ld * 2, left = to.bytes - skip;
+      const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(to.base + skip, left > 0 ? (unsigned)left : 0u);
+      __builtin_amdgcn_raw_buffer_store_b128(w, rsrc, (int)to.voff[q], 0, AUX);
+    };
+    // GATED: columns 2 e2 and 2 e2 + 1 of the lane's 8 in half q of row block i (blocks 4 q .. 4 q + 3 hold gate, up of the first
+    // four columns, gate, up of the others); the 8 leave with the last two.
+    i32x4 made = {0, 0, 0, 0};
+    auto gated_pair = [&](auto i_tag, auto q_tag, auto e_tag, auto last_tag) __attribute__((always_inline)) {
+      constexpr int i = decltype(i_tag)::value, q = decltype(q_tag)::value, e2 = decltype(e_tag)::value;
+      constexpr int R0 = 4 * (8 * i + 4 * q + 2 * (e2 >> 1)) + 2 * (e2 & 1);
+      typedef T pair_t __attribute__((ext_vector_type(2)));
+      const pair_t two = {(T)gated_f32<T>(w4_acc_read<R0>(), w4_acc_read<R0 + 4>()), (T)gated_f32<T>(w4_acc_read<R0 + 1>(), w4_acc_read<R0 + 5>())};
+      made[e2] = __builtin_bit_cast(int, two);
+      if constexpr (e2 == 3) gated_store(out, i_tag, q_tag, N, made, last_tag);
+    };
+    // ... the lane's 8 gate (up = 0) or up factors
+    auto gated_factor = [&](auto i_tag, auto q_tag, auto up_tag, auto last_tag) __attribute__((always_inline)) {
+      constexpr int up = decltype(up_tag)::value;
+      constexpr int R0 = 4 * (8 * decltype(i_tag)::value + 4 * decltype(q_tag)::value + up);
+      vec8 v;
+      v[0] = (T)w4_acc_read<R0 + 0>();
+      v[1] = (T)w4_acc_read<R0 + 1>();
+      v[2] = (T)w4_acc_read<R0 + 2>();
+      v[3] = (T)w4_acc_read<R0 + 3>();
+      v[4] = (T)w4_acc_read<R0 + 8>();
+      v[5] = (T)w4_acc_read<R0 + 9>();
+      v[6] = (T)w4_acc_read<R0 + 10>();
+      v[7] = (T)w4_acc_read<R0 + 11>();
+      gated_store(up ? out_up : out_gate, i_tag, q_tag, 2 * N, __builtin_bit_cast(i32x4, v), last_tag);
     };
 
     // ---- one K tile ------------------------------------------------------------------------------
@@ -568,7 +631,16 @@ struct GemmW4 {
         if constexpr (MX && gap >= 32 && gap < 48 && (gap & 3) == 0) turn_scales(std::integral_constant<int, (gap - 32) / 4>{});
         if constexpr (MX && gap >= 48 && gap < 56 && (gap & 1) == 0) load_scales(std::integral_constant<int, (gap - 48) / 2>{});
         if constexpr (MX && gap == 57) advance_scales();
-        if constexpr (FIRST && !LN && gap >= 10 && gap < 10 + 8 * FM && ((gap - 10) & 1) == 0) {
+        if constexpr (FIRST && GATED && gap >= 10 && gap < 10 + 8 * FM) {
+          using RowBlock = std::integral_constant<int, (gap - 10) / 8>;
+          if (out.bytes > 0)  // (uniform) not in front of a workgroup's first tile
+            gated_pair(RowBlock{}, std::integral_constant<int, (gap - 10) / 4 % 2>{}, std::integral_constant<int, (gap - 10) % 4>{}, std::false_type{});
+          // (a row block's factors may be read until step B comes to it, 54 gaps on; a store in every other gap)
+          if constexpr (gap % 2 == 0) {
+            if (out_gate.bytes > 0) gated_factor(RowBlock{}, std::integral_constant<int, (gap - 10) / 4 % 2>{}, std::integral_constant<int, (gap - 10) / 2 % 2>{}, std::false_type{});
+          }
+        }
+        if constexpr (FIRST && !LN && !GATED && gap >= 10 && gap < 10 + 8 * FM && ((gap - 10) & 1) == 0) {
           // pair q of row block i goes into gap 10 + 8 i + 2 q
           store_pair(std::integral_constant<int, (gap - 10) / 8>{}, std::integral_constant<int, ((gap - 10) / 2) % 4>{}, std::false_type{});
         }
@@ -663,13 +735,27 @@ struct GemmW4 {
         next_b = rows_of_b(j + 1, tc_cur);
         if constexpr (MX) next_scales(j + 1, tc_cur);
         k_tile(std::true_type{});
-        out = out_tile_of(j, tc_j);  // from here on the accumulators belong to tile j
+        if constexpr (GATED) {
+          out = gated_out(j, tc_j, p.C, N);
+          out_gate = gated_out(j, tc_j, p.gu, 2 * N);
+          out_up = gated_out(j, tc_j, p.gu ? (T*)p.gu + N : nullptr, 2 * N);
+        } else out = out_tile_of(j, tc_j);  // from here on the accumulators belong to tile j
         for (int h = 1; h < n_k; ++h) k_tile(std::false_type{});
       }
       // Drain, then the last tile's output.
       wait_vm_and_lds<0>();
       drain();
-      w4_static_for<0, FM * FN / 2>([&](auto o_tag) __attribute__((always_inline)) {
+      if constexpr (GATED) {
+        w4_static_for<0, FM * 2>([&](auto o_tag) __attribute__((always_inline)) {
+          using RowBlock = std::integral_constant<int, decltype(o_tag)::value / 2>;
+          using Half = std::integral_constant<int, decltype(o_tag)::value % 2>;
+          w4_static_for<0, 4>([&](auto e_tag) __attribute__((always_inline)) { gated_pair(RowBlock{}, Half{}, e_tag, std::true_type{}); });
+          if (p.gu) {
+            gated_factor(RowBlock{}, Half{}, std::integral_constant<int, 0>{}, std::true_type{});
+            gated_factor(RowBlock{}, Half{}, std::integral_constant<int, 1>{}, std::true_type{});
+          }
+        });
+      } else w4_static_for<0, FM * FN / 2>([&](auto o_tag) __attribute__((always_inline)) {
         constexpr int o = decltype(o_tag)::value;
         store_pair(std::integral_constant<int, o / 4>{}, std::integral_constant<int, o % 4>{}, std::true_type{});
       });
@@ -972,6 +1058,12 @@ struct GemmW4 {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 };
+
+template <typename T, int STORE>
+__global__ void __launch_bounds__(256) gemm_gated_w4_kernel(const GemmParams p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  GemmW4<T, STORE, false, 4, 8, 2, false, false, true>::run(p, smem);
+}
 
 template <typename T, int STORE>
 __global__ void __launch_bounds__(256) gemm_mx_w4_kernel(const MxW4Params p) {

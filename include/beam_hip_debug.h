@@ -70,8 +70,8 @@ size_t beam_dbg_ln_plan_bytes(int M, int N, int K, const beam_tile_cfg* cfg, int
  * (K % 8 == 0), 2 on 128 (K % 64 == 0).  Before a device has been probed, of one with 256 CUs. */
 int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, int* cols, int* waves, int* whole_lines);
 /* Measurement only: the tile that MXFP4 products, and gated layers, run on from now on, named as beam_dbg_mx_tile and
- * beam_dbg_gated_tile name it, whether it suits the problem or not; rows = 0: the library's choice again.  A tile that is not
- * compiled makes the calls fail. */
+ * beam_dbg_gated_tile name it, whether it is good for a problem or not; rows = 0: the library's choice again.  A tile that a problem
+ * cannot run on is not taken, one that is not compiled makes the calls fail. */
 int beam_dbg_set_mx_tile(int rows, int cols, int kwave);
 int beam_dbg_set_gated_tile(int rows, int cols, int kind);
 /* ... and how the products of a gated layer's backward pass are cut into K slices, in tiles of rows (64, 128) x 128; slices = 1: not at
@@ -81,7 +81,7 @@ int beam_dbg_set_nn_split(int rows, int slices);
  * 2 if a workgroup on each CU walks the tiles (C on 16 bytes). */
 int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave);
 /* What beam_gemmrc_gated runs an M x N x K problem on (K from 8 on): rows x cols rows of A and B, kind 0 tiles of gemm_kernel.h,
- * 2 the deep ones, 3 those that fill by whole lines, 4 tiles of gemm_kwave.h, 5 those that fill by whole lines.  row_starts as in
+ * 1 tiles that a workgroup on each CU walks (outputs on 16 bytes), 2 the deep ones, 3 those that fill by whole lines, 4 tiles of gemm_kwave.h, 5 those that fill by whole lines.  row_starts as in
  * beam_dbg_small_tile. */
 int beam_dbg_gated_tile(int M, int N, int K, int row_starts, int* rows, int* cols, int* kind);
 /* The tile that beam_gemmrc without one runs on where beam_dbg_small_tile says none and the rows of A and B start on 16 bytes

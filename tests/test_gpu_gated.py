@@ -22,10 +22,9 @@ TINY = {F16: 2.0 ** -24, BF16: 2.0 ** -126}
 
 # (rows, rows of B, kind) of beam_dbg_gated_tile -> problems that it names
 TILES = {
-    (8, 32, 4): [(1, 8, 9), (3, 70, 200), (8, 333, 64), (1, 1, 8)],
-    (8, 64, 4): [(1, 4135, 12), (5, 4267, 64)],
-    (16, 32, 4): [(9, 9, 15), (16, 300, 513), (10, 8, 64)],
-    (16, 64, 4): [(10, 4365, 10), (9, 4447, 64), (16, 5000, 200)],
+    (8, 32, 4): [(1, 8, 9), (3, 70, 200), (8, 333, 64), (1, 1, 8), (1, 4135, 12), (5, 4267, 64)],
+    (16, 32, 4): [(9, 9, 15), (16, 300, 513), (10, 8, 64), (10, 4365, 10), (9, 4447, 64), (16, 5000, 200)],
+    (16, 64, 4): [(40, 2700, 64), (37, 2125, 100)],
     (32, 32, 4): [(4144, 8, 13), (31, 4000, 64)],
     (32, 64, 4): [(4627, 17, 9), (17, 4167, 8), (19, 4697, 64)],
     (64, 32, 4): [(4469, 39, 17), (4193, 37, 64)],
@@ -46,6 +45,7 @@ TILES = {
     (192, 256, 0): [(4395, 948, 346), (1098, 3863, 344), (881, 4704, 384)],
     (224, 256, 0): [(1570, 3791, 122), (3592, 1699, 112), (2440, 2686, 128)],
     (256, 256, 0): [(3956, 1827, 164), (2246, 2957, 144), (2939, 2606, 192)],
+    (256, 256, 1): [(1812, 3992, 192), (4096, 2048, 192), (3877, 1944, 192)],
     (256, 128, 0): [(1930, 1105, 1487), (1062, 2005, 1472)],
     (128, 256, 0): [(1310, 2907, 2432)],
 }
@@ -150,7 +150,7 @@ def test_forward(gpu, beamc, oracle, tile):
         assert (again == h).all(), "h depends on whether gu is asked for"
         other = 1 - dtype
         a, b = inputs(beamc, M, N, K, other)
-        h, gu = run_forward(beamc, a, b, other, offsets=(1, 3, 1, 5) if i % 2 else (8, 24, 2, 4))
+        h, gu = run_forward(beamc, a, b, other, offsets=(1, 3, 8, 16) if tile[2] == 1 else (1, 3, 1, 5) if i % 2 else (8, 24, 2, 4))
         check_forward(oracle, a, b, h, gu, other, (tile, M, N, K, other, "anywhere"))
 
 
@@ -409,3 +409,20 @@ def test_backward_of_a_few_tokens_through_a_wide_layer(gpu, beamc, oracle):
         check_products(D.T, f64(oracle, a, BF16), f64(oracle, db, BF16), HALF_STEP[BF16], TINY[BF16], ("db", M, N, K))
         again = run_backward(beamc, dh, gu, a, b, BF16)
         assert (again[0] == da).all() and (again[1] == db).all()
+
+
+def test_walking_tiles_of_several_rounds(gpu, beamc, oracle):
+    """More 256 x 256 tiles than twice the CUs: every workgroup carries its sums through several tile boundaries."""
+    M, N, K = 6147, 2920, 320
+    beamc.lib.beam_dbg_set_gated_tile(256, 256, 1)
+    try:
+        assert tile_of(beamc, M, N, K) == (256, 256, 1)
+        a, b = inputs(beamc, M, N, K, BF16)
+        h, gu = run_forward(beamc, a, b, BF16)
+        check_forward(oracle, a, b, h, gu, BF16, (M, N, K))
+        assert (run_forward(beamc, a, b, BF16, train=False)[0] == h).all()
+        # outputs off 16 bytes, and K tiles that are not whole: not that kernel's
+        h, gu = run_forward(beamc, a[:300], b, BF16, offsets=(0, 0, 1, 0))
+        check_forward(oracle, a[:300], b, h, gu, BF16, "off 16 bytes")
+    finally:
+        beamc.lib.beam_dbg_set_gated_tile(0, 0, 0)
