@@ -1248,26 +1248,47 @@ int check_mx_product(const void* C, int M, int N, int K, int dtype) {
   return BEAM_OK;
 }
 
-// What an MXFP4 product runs on: rows x cols, the tile of gemm_mx.h's two kernels.
+// What an MXFP4 product runs on: rows x cols, a tile of the kernels of gemm_mx.h and gemm_w4.h.
 struct MxPlan {
   int rows, cols;
   int kwave;  // 1: K tiles dealt out to the wavefronts; 2: the kernel of gemm_w4.h
 };
 std::atomic<int> g_mx_rows{0}, g_mx_cols{0}, g_mx_kwave{0};  // beam_dbg_set_mx_tile
 MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
-  const bool w4_fits = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
-  if (const int rows = g_mx_rows.load(std::memory_order_relaxed); rows && (g_mx_kwave.load(std::memory_order_relaxed) != 2 || w4_fits))
+  // the walking kernel: whole K tiles, three and more
+  const bool walk = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
+  if (const int rows = g_mx_rows.load(std::memory_order_relaxed); rows && (g_mx_kwave.load(std::memory_order_relaxed) != 2 || walk))
     return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), g_mx_kwave.load(std::memory_order_relaxed)};
-  static const struct { int rows, cols; } kSmall[] = {{16, 16}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
+  // As in kw_plan the smallest sum of rows and columns of which the problem has at most one tile for every CU; a handful of rows
+  // takes 64 columns at a time however many tiles that makes (1 x 11008 x 4096 6.4 us, 32 columns 7.0, 16 6.7).  (64 x 64 is always
+  // behind the tiled kernel here, whose K loop is short: 512 x 4096 x 4096 13.2, 10.3 us; 366 x 2304 x 576 4.6, 3.7.)
+  static const struct { int rows, cols; } kSmall[] = {{16, 16}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}};
   auto tiles = [&](int r, int c) { return ((long)M + r - 1) / r * (((long)N + c - 1) / c); };
   for (const auto& t : kSmall) {
     const bool few = M <= 16 && t.rows == 16 && t.cols == 64;
     if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, 1};
   }
-  if (tiles(256, 256) >= cus) return MxPlan{256, 256, w4_fits ? 2 : 0};
-  if (tiles(256, 128) >= cus) return MxPlan{256, 128, 0};
-  if (tiles(128, 128) >= cus) return MxPlan{128, 128, 0};
-  return MxPlan{64, 64, 0};
+  // The others by rounds of workgroups, each with a start and an end and its K tiles; us, from timings of shapes from 175 x 4480 x
+  // 288 to 8192^3.  (64 x 64: two workgroups to a CU, and faster alone.)
+  struct Candidate {
+    MxPlan plan;
+    int per_cu;
+    double fixed, k_tile;
+  };
+  const bool alone = tiles(64, 64) <= cus;
+  const Candidate kTiles[] = {{{64, 64, 0}, 2, alone ? 0.7 : 1.5, alone ? 0.17 : 0.38},
+                              {{128, 128, 0}, 1, 2.4, 0.70},
+                              {{256, 128, 0}, 1, 4.0, 1.06},
+                              {{256, 256, walk ? 2 : 0}, 1, walk ? 4.0 : 6.0, walk ? 1.78 : 2.0}};
+  const int k_tiles = (K + kMxTile - 1) / kMxTile;
+  MxPlan best = kTiles[0].plan;
+  double best_us = 1e300;
+  for (const Candidate& c : kTiles) {
+    const long slots = (long)cus * c.per_cu, rounds = (tiles(c.plan.rows, c.plan.cols) + slots - 1) / slots;
+    const double us = (double)rounds * (c.fixed + c.k_tile * k_tiles);
+    if (us < best_us) best_us = us, best = c.plan;
+  }
+  return best;
 }
 
 int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* sB, void* C, int M, int N, int K, int dtype, hipStream_t st) {

@@ -126,8 +126,7 @@ __device__ __forceinline__ i32x4 mx_encode_block(const V8 (&x)[4], int* scale) {
   X(16, 64, 4)                    \
   X(32, 32, 4)                    \
   X(32, 64, 4)                    \
-  X(64, 32, 4)                    \
-  X(64, 64, 4)
+  X(64, 32, 4)
 template <typename T>
 hipError_t launch_gemm_mx(int block_m, int block_n, const MxParams& p, hipStream_t stream);
 template <> hipError_t launch_gemm_mx<_Float16>(int, int, const MxParams&, hipStream_t);

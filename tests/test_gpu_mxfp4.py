@@ -191,7 +191,7 @@ def run_product(beamc, a, b, dtype, offset=0, behind=0xFF):
     return got
 
 
-# (rows, columns, kwave) of beam_dbg_mx_tile -> (M, N)
+# (rows, columns, kwave) of beam_dbg_mx_tile -> (M, N) that it names at K = 1024
 TILES = {
     (16, 16, 1): [(1, 1), (1, 300), (16, 4096), (77, 100)],
     (16, 32, 1): [(9, 4133), (200, 345)],
@@ -199,12 +199,11 @@ TILES = {
     (32, 32, 1): [(500, 493)],
     (32, 64, 1): [(500, 1003)],
     (64, 32, 1): [(9000, 20)],
-    (64, 64, 1): [(1000, 1001), (1024, 1024)],
-    (64, 64, 0): [(1500, 1001), (129, 9000)],
-    (128, 128, 0): [(2040, 2049), (700, 6001)],
-    (256, 128, 0): [(4001, 2101), (4096, 2048)],
-    (256, 256, 0): [(4097, 3901), (4000, 4090)],
-    (256, 256, 2): [(4097, 3904), (4096, 4096), (8200, 4104)],
+    (64, 64, 0): [(1000, 1001), (1024, 1024), (129, 9000)],
+    (128, 128, 0): [(200, 8531), (194, 8653)],
+    (256, 128, 0): [(515, 7513), (6673, 578)],
+    (256, 256, 0): [(835, 9511), (6303, 1283)],
+    (256, 256, 2): [(918, 8304), (4644, 1696), (8200, 4104)],
 }
 
 
@@ -224,13 +223,18 @@ def test_problems_reach_the_tiles_that_they_are_listed_under(gpu, beamc):
 @pytest.mark.parametrize("K", [32, 224, 256, 288, 544, 1024, 2016])
 def test_product(gpu, beamc, oracle, tile, K):
     rng = np.random.default_rng(K)
-    for i, (M, N) in enumerate(TILES[tile]):
-        if M * N > 1 << 22 and (K > 1024 or (tile[2] == 2) != (K == 1024)):
-            continue  # (the walking kernel is for whole K tiles, three and more)
-        dtype, offset = ((F16, 0), (BF16, 0 if tile[2] == 2 else 1))[(i + K // 32) % 2]
-        a, b = operand(rng, M, K), operand(rng, N, K)
-        got = run_product(beamc, a, b, dtype, offset)
-        check_product(oracle, held(*a), held(*b), got, dtype, (tile, M, N, K, dtype))
+    beamc.lib.beam_dbg_set_mx_tile(*tile)  # at every K, not only where it is the best
+    try:
+        for i, (M, N) in enumerate(TILES[tile]):
+            if M * N > 1 << 22 and K > 1024 or tile[2] == 2 and K != 1024:
+                continue  # (the walking kernel is for whole K tiles, three and more)
+            dtype, offset = ((F16, 0), (BF16, 0 if tile[2] == 2 else 1))[(i + K // 32) % 2]
+            a, b = operand(rng, M, K), operand(rng, N, K)
+            assert tile_of(beamc, M, N, K) == tile
+            got = run_product(beamc, a, b, dtype, offset)
+            check_product(oracle, held(*a), held(*b), got, dtype, (tile, M, N, K, dtype))
+    finally:
+        beamc.lib.beam_dbg_set_mx_tile(0, 0, 0)
 
 
 def test_product_of_nothing(gpu, beamc):
