@@ -1268,8 +1268,10 @@ MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
     const bool few = M <= 16 && t.rows == 16 && t.cols == 64;
     if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, 1};
   }
-  // The others by rounds of workgroups, each with a start and an end and its K tiles; us, from timings of shapes from 175 x 4480 x
-  // 288 to 8192^3.  (64 x 64: two workgroups to a CU, and faster alone.)
+  // The others by rounds of workgroups, each with a start and an end and its K tiles; us, from timings of 40 shapes from 175 x 4480 x
+  // 288 to 8192^3, on most of which the pick is the best tile; 1500 x 1500 x 1504 is furthest, 10.4 us against 9.2 in 64 x 64 tiles.  (64 x 64: two workgroups to a CU, and faster alone.  The
+  // walking kernel keeps more in flight and starts later: 8192^3 233 us against 268 with one workgroup per tile, 4096^3 35, 40; in two
+  // rounds under short sums the others are ahead, 7698 x 3456 x 768 29.5, 24.0, x 1536 38.8, 35.8.)
   struct Candidate {
     MxPlan plan;
     int per_cu;
@@ -1279,11 +1281,13 @@ MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
   const Candidate kTiles[] = {{{64, 64, 0}, 2, alone ? 0.7 : 1.5, alone ? 0.17 : 0.38},
                               {{128, 128, 0}, 1, 2.4, 0.70},
                               {{256, 128, 0}, 1, 4.0, 1.06},
-                              {{256, 256, walk ? 2 : 0}, 1, walk ? 4.0 : 6.0, walk ? 1.78 : 2.0}};
+                              {{256, 256, 0}, 1, 5.0, 1.95},
+                              {{256, 256, 2}, 1, tiles(256, 256) <= cus ? 5.0 : 8.5, 1.5}};
   const int k_tiles = (K + kMxTile - 1) / kMxTile;
   MxPlan best = kTiles[0].plan;
   double best_us = 1e300;
   for (const Candidate& c : kTiles) {
+    if (c.plan.kwave == 2 && !walk) continue;
     const long slots = (long)cus * c.per_cu, rounds = (tiles(c.plan.rows, c.plan.cols) + slots - 1) / slots;
     const double us = (double)rounds * (c.fixed + c.k_tile * k_tiles);
     if (us < best_us) best_us = us, best = c.plan;
@@ -1318,6 +1322,7 @@ int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* s
   p.tiles_m = (M + plan.rows - 1) / plan.rows;
   p.tiles_n = (N + plan.cols - 1) / plan.cols;
   p.group_m = plan.kwave ? 8 : default_group_m(plan.rows, plan.cols);
+  p.c_store = store_kind(beam_tile_cfg{plan.rows, plan.cols, 0, 0, 0, 0}, 4, false, C, M, N, K / 4);
   p.divs = make_tile_divs(p.tiles_m, p.tiles_n, p.group_m);
   if (plan.kwave) BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx_kwave<_Float16>(plan.rows, plan.cols, a16, p, st) : launch_gemm_mx_kwave<__bf16>(plan.rows, plan.cols, a16, p, st));
   else BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx<_Float16>(plan.rows, plan.cols, p, st) : launch_gemm_mx<__bf16>(plan.rows, plan.cols, p, st));

@@ -270,13 +270,48 @@ struct MxGemm {
       mx_multiply_row<1, decltype(i_tag)::value>(fa1[decltype(i_tag)::value], fb1, sa, sb, acc[decltype(i_tag)::value]);
     });
     wait_vm_and_lds<0>();  // (fills behind the last K tile)
+    __syncthreads();       // every slot is dead
+    // Through LDS, as in gemm_kernel.h, whose layout this is: 16 bytes a lane, whole rows of the wavefront's part at a time (7698 x
+    // 3456 x 256, 8 bytes a lane straight from the sums 26 us, so 17.6).
+    constexpr int RB = TN * 2, LPR = TN / 8, RPI = 64 / LPR;
+    static_assert(NW * TM * RB <= LDS_BYTES && (RB == 64 || RB == 128), "staging area");
+    auto chunk_xor = [](int row) { return RB == 64 ? (row >> 1) & 3 : row & 7; };
+    // (the lane's constants here from a value that the compiler cannot see through: hoisted in front of the K loop they cost the
+    // 256 x 256 tile registers that it does not have, 2048 x 4096 x 11008 78 -> 87 us)
+    int ol = lane;
+    asm volatile("" : "+v"(ol));
+    const int wr = ol & 15, wg = ol >> 4;
+    char* const stage = smem + wave * (TM * RB);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int m = row0 + wm * TM + i * 16 + r;
-      if (m >= M) continue;
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) mx_store_quad((T*)p.C + (size_t)m * N, col0 + wn * TN + j * 16 + 4 * g, N, acc[i][j]);
-    }
+      for (int j = 0; j < FN; ++j) {
+        typename ElemTraits<T>::vec4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)acc[i][j][e];
+        *(typename ElemTraits<T>::vec4*)(stage + (i * 16 + wr) * RB + (((wg & 1) ^ (wr >> 3)) << 3) + (((2 * j + (wg >> 1)) ^ chunk_xor(wr)) << 4)) = v;
+      }
+    using vec8 = typename ElemTraits<T>::vec8;
+    const int srow = ol / LPR, schunk = ol % LPR;
+    auto store_all = [&](auto kind_tag) __attribute__((always_inline)) {
+#pragma unroll
+      for (int it = 0; it < TM / RPI; ++it) {
+        const int row = it * RPI + srow;
+        vec8 v = *(const vec8*)(stage + row * RB + schunk * 16);
+        if ((row >> 3) & 1) v = vec8{v[4], v[5], v[6], v[7], v[0], v[1], v[2], v[3]};
+        const int m = row0 + wm * TM + row, n = col0 + wn * TN + (schunk ^ chunk_xor(row)) * 8;
+        T* const at = (T*)p.C + (size_t)m * N + n;
+        if (m < M && n + 7 < N) {
+          store_16<decltype(kind_tag)::value>(at, __builtin_bit_cast(i32x4, v));
+        } else if (m < M && n < N) {
+#pragma unroll
+          for (int e = 0; e < 7; ++e)
+            if (n + e < N) at[e] = v[e];
+        }
+      }
+    };
+    if (p.c_store == kStoreThrough) store_all(std::integral_constant<int, kStoreThrough>{});
+    else store_all(std::integral_constant<int, kStoreCached>{});
   }
 };
 

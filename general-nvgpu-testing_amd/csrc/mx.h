@@ -38,6 +38,7 @@ struct MxParams {
   int M, N, K;
   int tiles_m, tiles_n, group_m;
   TileDivs divs;
+  int c_store;  // StoreKind of the tiled kernel
 };
 
 // Where chunk c of a row's 8 lies in LDS before the row's XOR: lane group g reads place 4 step + g, as of 16-bit elements, for

@@ -191,7 +191,7 @@ def run_product(beamc, a, b, dtype, offset=0, behind=0xFF):
     return got
 
 
-# (rows, columns, kwave) of beam_dbg_mx_tile -> (M, N) that it names at K = 1024
+# (rows, columns, kwave) of beam_dbg_mx_tile -> (M, N) that it names at K = 1024, for the walking kernel 4096
 TILES = {
     (16, 16, 1): [(1, 1), (1, 300), (16, 4096), (77, 100)],
     (16, 32, 1): [(9, 4133), (200, 345)],
@@ -216,7 +216,8 @@ def tile_of(beamc, M, N, K):
 def test_problems_reach_the_tiles_that_they_are_listed_under(gpu, beamc):
     for tile, problems in TILES.items():
         for M, N in problems:
-            assert tile_of(beamc, M, N, 1024) == tile, (M, N, tile_of(beamc, M, N, 1024))
+            K = 4096 if tile[2] == 2 else 1024
+            assert tile_of(beamc, M, N, K) == tile, (M, N, tile_of(beamc, M, N, K))
 
 
 @pytest.mark.parametrize("tile", sorted(TILES), ids=lambda t: "x".join(map(str, t)))
