@@ -1228,6 +1228,7 @@ int check_mx(int rows, int K, int dtype) {
   if (K % 32 != 0) return fail(BEAM_ERR_INVALID, "K=%d is not a whole number of blocks of 32", K);
   if (K > kMxMaxK) return fail(BEAM_ERR_UNSUPPORTED, "K=%d beyond %d", K, kMxMaxK);
   if (dtype != BEAM_F16 && dtype != BEAM_BF16) return fail(BEAM_ERR_UNSUPPORTED, "dtype %d: only fp16 (0) and bf16 (1)", dtype);
+  if (((long)rows + 31) / 32 * (((long)K + kMxTile - 1) / kMxTile) > INT32_MAX) return fail(BEAM_ERR_UNSUPPORTED, "%d rows of K=%d are too many", rows, K);
   return BEAM_OK;
 }
 
@@ -1254,11 +1255,14 @@ struct MxPlan {
   int kwave;  // 1: K tiles dealt out to the wavefronts; 2: the kernel of gemm_w4.h
 };
 std::atomic<int> g_mx_rows{0}, g_mx_cols{0}, g_mx_kwave{0};  // beam_dbg_set_mx_tile
-MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
+// a16: A is 16-bit, M at most 16 (a tile of 16 rows of gemm_mx.h's small ones, which the rule below names for any such M).
+MxPlan mx_plan(int M, int N, int K, const void* C, bool a16, int cus) {
   // the walking kernel: whole K tiles, three and more
   const bool walk = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
-  if (const int rows = g_mx_rows.load(std::memory_order_relaxed); rows && (g_mx_kwave.load(std::memory_order_relaxed) != 2 || walk))
-    return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), g_mx_kwave.load(std::memory_order_relaxed)};
+  if (const int rows = g_mx_rows.load(std::memory_order_relaxed)) {
+    const int kind = g_mx_kwave.load(std::memory_order_relaxed);
+    if (a16 ? kind == 1 && rows == 16 : kind != 2 || walk) return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), kind};
+  }
   // As in kw_plan the smallest sum of rows and columns of which the problem has at most one tile for every CU; a handful of rows
   // takes 64 columns at a time however many tiles that makes (1 x 11008 x 4096 6.4 us, 32 columns 7.0, 16 6.7).  (64 x 64 is always
   // behind the tiled kernel here, whose K loop is short: 512 x 4096 x 4096 13.2, 10.3 us; 366 x 2304 x 576 4.6, 3.7.)
@@ -1297,7 +1301,7 @@ MxPlan mx_plan(int M, int N, int K, const void* C, int cus) {
 
 int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* sB, void* C, int M, int N, int K, int dtype, hipStream_t st) {
   const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
-  const MxPlan plan = mx_plan(M, N, K, C, cus);
+  const MxPlan plan = mx_plan(M, N, K, C, a16, cus);
   if (plan.kwave == 2) {
     const beam_tile_cfg c = {256, 256, 128, 128, 0, default_group_m(256, 256)};
     MxW4Params p;
@@ -2219,7 +2223,7 @@ int beam_dbg_set_gated_tile(int rows, int cols, int kind) {
 
 int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave) {
   if (!rows || !cols || !kwave || M < 1 || N < 1 || K < 32) return fail(BEAM_ERR_INVALID, "arguments");
-  const MxPlan plan = mx_plan(M, N, K, nullptr, g_dev.cus > 0 ? g_dev.cus : 256);
+  const MxPlan plan = mx_plan(M, N, K, nullptr, false, g_dev.cus > 0 ? g_dev.cus : 256);
   *rows = plan.rows, *cols = plan.cols, *kwave = plan.kwave;
   return BEAM_OK;
 }

@@ -270,7 +270,7 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
 int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, void* stream);
 
 /* The gradients of that layer: with s = 1 / (1 + exp(-G)), D = [dH * U * s * (1 + G * (1 - s)), dH * G * s] ([M][2N], rounded to
- * the dtype for the products that follow), dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or
+ * the dtype for the products that follow: in fp16 infinite beyond 65504 and coarse below 2^-14, as any gradient held in fp16), dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or
  * dB may be null: not asked for.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches, and one more for a
  * product of so few outputs that its sums are cut into slices, which are added in their order; the workspace (256-byte
  * aligned, any contents) holds D, its transpose and such sums, and belongs to the call until it has run: calls that overlap in time need one

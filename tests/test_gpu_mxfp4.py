@@ -291,6 +291,23 @@ def test_linear(gpu, beamc, oracle, M):
             t.free()
 
 
+def test_linear_is_not_misled_by_a_named_tile(gpu, beamc, oracle):
+    """beam_dbg_set_mx_tile names tiles for operands in MXFP4; 16-bit rows keep to those that take them."""
+    M, N, K = 5, 300, 256
+    bits = beamc.host_normal((M, K), BF16, 16, 0, 0.0, 1.0)
+    b = operand(np.random.default_rng(4), N, K)
+    x, q, s, c = Guarded(beamc, bits, 0, BF16), Bytes(beamc, packed(b[0])), Bytes(beamc, to_tiles(b[1])), Guarded(beamc, (M, N), 0, BF16)
+    for tile in ((64, 64, 0), (32, 64, 1), (16, 16, 1), (16, 64, 1)):
+        beamc.lib.beam_dbg_set_mx_tile(*tile)
+        try:
+            beamc._check(beamc.lib.beam_linear_mxfp4(x.ptr, q.ptr, s.ptr, c.ptr, M, N, K, BF16, None, 0, None))
+        finally:
+            beamc.lib.beam_dbg_set_mx_tile(0, 0, 0)
+        check_product(oracle, held(*quantized(f64(oracle, bits, BF16))), held(*b), c.read(), BF16, tile)
+    for t in (x, q, s, c):
+        t.free()
+
+
 def test_linear_of_a_token_with_a_nan(gpu, beamc, oracle):
     M, N, K = 3, 100, 512
     bits = beamc.host_normal((M, K), BF16, 14, 0, 0.0, 1.0)

@@ -23,6 +23,7 @@ def test_quantize_and_dequantize(beamc):
         refused(beamc, call(K=48), INVALID, "blocks of 32")
         refused(beamc, call(K=(1 << 22) + 32), UNSUPPORTED, "beyond")
         refused(beamc, call(dtype=F32), UNSUPPORTED, "dtype")
+        refused(beamc, call(rows=(1 << 31) - 1, K=1 << 22), UNSUPPORTED, "too many")
         refused(beamc, call(x=None), INVALID, "null")
         refused(beamc, call(q=None), INVALID, "null")
         refused(beamc, call(s=None), INVALID, "null")
