@@ -10,7 +10,6 @@
 
 namespace beam {
 
-
 // A workgroup tile of the gated kernel: block_n rows of B, half of them gate and half up rows, so block_n / 2 columns of C.
 enum GatedDepth : int { kGatedShallow = 0, kGatedWalk = 1, kGatedDeep = 2, kGatedLines = 3 };
 struct GatedTile {

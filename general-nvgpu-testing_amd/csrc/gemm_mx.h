@@ -112,7 +112,7 @@ __device__ __forceinline__ void mx_store_quad(T* row, int n, int N, f32x4 v) {
 // The K loop is gemm_kernel.h's: while the MFMAs of one half of a K tile run, the fragments of the next half are read, a few
 // between the MFMAs of each row, and the fills of the K tile ST - 1 further on are issued, a row's share behind each row; of two
 // wavefronts on a SIMD the older one issues all of them.  A row is closed by a scheduling fence: left alone, the compiler reads
-// every fragment right in front of the MFMA that needs it (MEASURED_PIPELINE).
+// every fragment right in front of the MFMA that needs it (8192^3 298 us, so 270).
 template <typename T, int BM, int BN, int WVM, int WVN, int ST>
 struct MxGemm {
   static constexpr int NW = WVM * WVN, NT = NW * 64;

@@ -43,7 +43,7 @@ struct MxParams {
 
 // Where chunk c of a row's 8 lies in LDS before the row's XOR: lane group g reads place 4 step + g, as of 16-bit elements, for
 // which that XOR is made (chunks 2 g + step in their own places: a read's groups of lanes meet in the same banks, 8192^3
-// CONFLICTS us).  A fill has each lane fetch the chunk that belongs where it writes, from the same line.
+// 241 us, so 235).  A fill has each lane fetch the chunk that belongs where it writes, from the same line.
 BEAM_HD int mx_place_of(int chunk) { return (chunk & 1) << 2 | chunk >> 1; }
 BEAM_HD int mx_chunk_at(int place) { return (place & 3) << 1 | place >> 2; }
 
@@ -114,8 +114,8 @@ __device__ __forceinline__ i32x4 mx_encode_block(const V8 (&x)[4], int* scale) {
   return o;
 }
 
-// Launchers.  gemm_mx: a tile of the tables below, {rows, columns}; gemm_mx_kwave: {rows, columns, wavefronts}, a16: p.A is 16-bit
-// and extra_lds bytes hold its elements (mx_kept_bytes).
+// Launchers.  Tiles of MxGemm: (rows, columns, wavefronts along M and N, LDS slots); of MxKw: (rows, columns, wavefronts), those of 16
+// rows also with a16: p.A is 16-bit and K at most kMxKeptColumns.
 #define BEAM_FOR_EACH_MX_TILE(X) \
   X(64, 64, 2, 2, 4)             \
   X(128, 128, 2, 2, 4)           \

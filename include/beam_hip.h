@@ -270,11 +270,12 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
 int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, void* stream);
 
 /* The gradients of that layer: with s = 1 / (1 + exp(-G)), D = [dH * U * s * (1 + G * (1 - s)), dH * G * s] ([M][2N], rounded to
- * the dtype for the products that follow: in fp16 infinite beyond 65504 and coarse below 2^-14, as any gradient held in fp16), dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or
- * dB may be null: not asked for.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches, and one more for a
+ * the dtype for the products that follow: in fp16 infinite beyond 65504 and coarse below 2^-14, as any gradient held in fp16),
+ * dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or dB may be null: not asked for; they overlap
+ * neither each other nor an input.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches, and one more for a
  * product of so few outputs that its sums are cut into slices, which are added in their order; the workspace (256-byte
- * aligned, any contents) holds D, its transpose and such sums, and belongs to the call until it has run: calls that overlap in time need one
- * each, and so does a captured graph that may run beside another. */
+ * aligned, any contents) holds D, its transpose and such sums, and belongs to the call until it has run: calls that overlap in
+ * time need one each, and so does a captured graph that may run beside another. */
 size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int K, int want_dA, int want_dB);
 int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
                                int dtype, void* ws, size_t ws_bytes, void* stream);
@@ -289,8 +290,9 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
  * No counterpart in the reference, whose operands are fp16. */
 size_t beam_mxfp4_scale_bytes(int rows, int K);
 /* X [rows][K] (16-bit, any element's address) in that format: a block's power of two is the one at or below its largest magnitude,
- * over 4 (at least 2^-127); an element is the nearest value of the eight, ties to the even code, 6 beyond 6.  A block with an infinity or a NaN
- * in it gets the scale NaN, and is NaN in whatever is made of it. */
+ * over 4 (at least 2^-127); an element is the nearest value of the eight, ties to the even code, 6 beyond 6.  A block with an
+ * infinity or a NaN in it gets the scale NaN, and is NaN in whatever is made of it.  Here and in the calls below, outputs overlap no
+ * input. */
 int beam_mxfp4_quantize(const void* X, void* elements, void* scales, int rows, int K, int dtype, void* stream);
 /* The values held, in dtype (rounded to nearest where it cannot hold them). */
 int beam_mxfp4_dequantize(const void* elements, const void* scales, void* X, int rows, int K, int dtype, void* stream);

@@ -81,8 +81,8 @@ int beam_dbg_set_nn_split(int rows, int slices);
  * 2 if a workgroup on each CU walks the tiles (C on 16 bytes). */
 int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave);
 /* What beam_gemmrc_gated runs an M x N x K problem on (K from 8 on): rows x cols rows of A and B, kind 0 tiles of gemm_kernel.h,
- * 1 tiles that a workgroup on each CU walks (outputs on 16 bytes), 2 the deep ones, 3 those that fill by whole lines, 4 tiles of gemm_kwave.h, 5 those that fill by whole lines.  row_starts as in
- * beam_dbg_small_tile. */
+ * 1 tiles that a workgroup on each CU walks (outputs on 16 bytes), 2 the deep ones, 3 those that fill by whole lines, 4 tiles of
+ * gemm_kwave.h, 5 those that fill by whole lines.  row_starts as in beam_dbg_small_tile. */
 int beam_dbg_gated_tile(int M, int N, int K, int row_starts, int* rows, int* cols, int* kind);
 /* The tile that beam_gemmrc without one runs on where beam_dbg_small_tile says none and the rows of A and B start on 16 bytes
  * but not on 128 (K % 64 != 0), and whether its fills take whole 128-byte lines (*whole_lines = 1: such a tile need not be in
