@@ -1252,16 +1252,16 @@ int check_mx_product(const void* C, int M, int N, int K, int dtype) {
 // What an MXFP4 product runs on: rows x cols, a tile of the kernels of gemm_mx.h and gemm_w4.h.
 struct MxPlan {
   int rows, cols;
-  int kwave;  // 1: K tiles dealt out to the wavefronts; 2: the kernel of gemm_w4.h
+  int kind;  // MxKind
 };
-std::atomic<int> g_mx_rows{0}, g_mx_cols{0}, g_mx_kwave{0};  // beam_dbg_set_mx_tile
+std::atomic<int> g_mx_rows{0}, g_mx_cols{0}, g_mx_kind{0};  // beam_dbg_set_mx_tile
 // a16: A is 16-bit, M at most 16 (a tile of 16 rows of gemm_mx.h's small ones, which the rule below names for any such M).
 MxPlan mx_plan(int M, int N, int K, const void* C, bool a16, int cus) {
   // the walking kernel: whole K tiles, three and more
   const bool walk = K % kMxTile == 0 && K / 4 >= kW4MinK && N % 8 == 0 && ((uintptr_t)C & 15) == 0 && N <= (1 << 21);
   if (const int rows = g_mx_rows.load(std::memory_order_relaxed)) {
-    const int kind = g_mx_kwave.load(std::memory_order_relaxed);
-    if (a16 ? kind == 1 && rows == 16 : kind != 2 || walk) return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), kind};
+    const int kind = g_mx_kind.load(std::memory_order_relaxed);
+    if (a16 ? kind == kMxKwave && rows == 16 : kind != kMxWalk || walk) return MxPlan{rows, g_mx_cols.load(std::memory_order_relaxed), kind};
   }
   // As in kw_plan the smallest sum of rows and columns of which the problem has at most one tile for every CU; a handful of rows
   // takes 64 columns at a time however many tiles that makes (1 x 11008 x 4096 6.4 us, 32 columns 7.0, 16 6.7).  (64 x 64 is always
@@ -1270,30 +1270,35 @@ MxPlan mx_plan(int M, int N, int K, const void* C, bool a16, int cus) {
   auto tiles = [&](int r, int c) { return ((long)M + r - 1) / r * (((long)N + c - 1) / c); };
   for (const auto& t : kSmall) {
     const bool few = M <= 16 && t.rows == 16 && t.cols == 64;
-    if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, 1};
+    if (tiles(t.rows, t.cols) <= cus || few) return MxPlan{t.rows, t.cols, kMxKwave};
   }
-  // The others by rounds of workgroups, each with a start and an end and its K tiles; us, from timings of 40 shapes from 175 x 4480 x
-  // 288 to 8192^3, on most of which the pick is the best tile; 1500 x 1500 x 1504 is furthest, 10.4 us against 9.2 in 64 x 64
-  // tiles.  (64 x 64: two workgroups to a CU, and faster alone.  The walking kernel keeps more in flight and starts later: 8192^3 233 us against 268 with one workgroup per tile, 4096^3 35, 40; in two
-  // rounds under short sums the others are ahead, 7698 x 3456 x 768 29.5, 24.0, x 1536 38.8, 35.8.)
+  // The others by rounds of workgroups, each with a start and an end and its K tiles, apart for a workgroup that has a CU to itself.
+  // us, fitted to timings of every tile on 158 shapes from 71 x 5200 x 384 to 8192^3: the picks are 0.3% behind the best tile on
+  // average and 10% at worst, 6582 x 192 x 6656.  Each is the best on some: 1024 x 4096 x 4096 12.7 us in 128 x 128 alone, 14.2 in 128 x
+  // 64, 15.7 in 128 x 128 by two, 16.0 in 256 x 128; 731 x 2448 x 6304 14.3 in 128 x 64, 16.7 in 64 x 64; 3044 x 6016 x 1376 28.8 in 128
+  // x 128 by two, 32.1 in 256 x 128; 2048 x 4096 x 11008 50.6 in 256 x 128, 57.9 in 128 x 128, 62.3 walking; 8192^3 239 walking, 278 in
+  // 256 x 256 with a workgroup per tile.  Two lengths of the ring of 64 x 64: 256 x 4096 x 11008 15.9 us in four slots, 18.4 in three;
+  // 1500 x 1500 x 1504 9.2, 8.2.
   struct Candidate {
     MxPlan plan;
     int per_cu;
-    double fixed, k_tile;
+    double fixed, k_tile, alone_fixed, alone_k_tile;
   };
-  const bool alone = tiles(64, 64) <= cus;
-  const Candidate kTiles[] = {{{64, 64, 0}, 2, alone ? 0.7 : 1.5, alone ? 0.17 : 0.38},
-                              {{128, 128, 0}, 1, 2.4, 0.70},
-                              {{256, 128, 0}, 1, 4.0, 1.06},
-                              {{256, 256, 0}, 1, 5.0, 1.95},
-                              {{256, 256, 2}, 1, tiles(256, 256) <= cus ? 5.0 : 8.5, 1.5}};
+  static const Candidate kTiles[] = {{{64, 64, kMxAlone}, 1, 1.1, 0.23, 1.0, 0.32},
+                                     {{64, 64, kMxShared}, 3, 1.9, 0.60, 0.5, 0.33},
+                                     {{128, 64, kMxShared}, 2, 2.6, 0.70, 2.0, 0.38},
+                                     {{128, 128, kMxAlone}, 1, 3.0, 0.57, 3.4, 0.49},
+                                     {{128, 128, kMxShared}, 2, 2.1, 1.23, 2.5, 0.82},
+                                     {{256, 128, kMxAlone}, 1, 4.5, 0.96, 3.6, 0.94},
+                                     {{256, 256, kMxAlone}, 1, 5.8, 2.11, 5.8, 1.82},
+                                     {{256, 256, kMxWalk}, 1, 6.5, 1.44, 7.1, 1.46}};
   const int k_tiles = (K + kMxTile - 1) / kMxTile;
   MxPlan best = kTiles[0].plan;
   double best_us = 1e300;
   for (const Candidate& c : kTiles) {
-    if (c.plan.kwave == 2 && !walk) continue;
-    const long slots = (long)cus * c.per_cu, rounds = (tiles(c.plan.rows, c.plan.cols) + slots - 1) / slots;
-    const double us = (double)rounds * (c.fixed + c.k_tile * k_tiles);
+    if (c.plan.kind == kMxWalk && !walk) continue;
+    const long n = tiles(c.plan.rows, c.plan.cols), slots = (long)cus * c.per_cu;
+    const double us = n <= cus ? c.alone_fixed + c.alone_k_tile * k_tiles : (double)((n + slots - 1) / slots) * (c.fixed + c.k_tile * k_tiles);
     if (us < best_us) best_us = us, best = c.plan;
   }
   return best;
@@ -1302,7 +1307,7 @@ MxPlan mx_plan(int M, int N, int K, const void* C, bool a16, int cus) {
 int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* sB, void* C, int M, int N, int K, int dtype, hipStream_t st) {
   const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
   const MxPlan plan = mx_plan(M, N, K, C, a16, cus);
-  if (plan.kwave == 2) {
+  if (plan.kind == kMxWalk) {
     const beam_tile_cfg c = {256, 256, 128, 128, 0, default_group_m(256, 256)};
     MxW4Params p;
     static_cast<GemmParams&>(p) = base_params(A, B, M, N, K / 4, c);
@@ -1325,11 +1330,11 @@ int run_mx(const void* A, const void* sA, bool a16, const void* B, const void* s
   p.K = K;
   p.tiles_m = (M + plan.rows - 1) / plan.rows;
   p.tiles_n = (N + plan.cols - 1) / plan.cols;
-  p.group_m = plan.kwave ? 8 : default_group_m(plan.rows, plan.cols);
+  p.group_m = plan.kind == kMxKwave ? 8 : default_group_m(plan.rows, plan.cols);
   p.c_store = store_kind(beam_tile_cfg{plan.rows, plan.cols, 0, 0, 0, 0}, 4, false, C, M, N, K / 4);
   p.divs = make_tile_divs(p.tiles_m, p.tiles_n, p.group_m);
-  if (plan.kwave) BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx_kwave<_Float16>(plan.rows, plan.cols, a16, p, st) : launch_gemm_mx_kwave<__bf16>(plan.rows, plan.cols, a16, p, st));
-  else BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx<_Float16>(plan.rows, plan.cols, p, st) : launch_gemm_mx<__bf16>(plan.rows, plan.cols, p, st));
+  if (plan.kind == kMxKwave) BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx_kwave<_Float16>(plan.rows, plan.cols, a16, p, st) : launch_gemm_mx_kwave<__bf16>(plan.rows, plan.cols, a16, p, st));
+  else BEAM_HIP(dtype == BEAM_F16 ? launch_gemm_mx<_Float16>(plan.rows, plan.cols, plan.kind, p, st) : launch_gemm_mx<__bf16>(plan.rows, plan.cols, plan.kind, p, st));
   return BEAM_OK;
 }
 
@@ -2199,10 +2204,10 @@ int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, 
   return BEAM_OK;
 }
 
-int beam_dbg_set_mx_tile(int rows, int cols, int kwave) {
+int beam_dbg_set_mx_tile(int rows, int cols, int kind) {
   g_mx_rows.store(0);
   g_mx_cols.store(cols);
-  g_mx_kwave.store(kwave);
+  g_mx_kind.store(kind);
   g_mx_rows.store(rows);
   return BEAM_OK;
 }
@@ -2221,10 +2226,10 @@ int beam_dbg_set_gated_tile(int rows, int cols, int kind) {
   return BEAM_OK;
 }
 
-int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave) {
-  if (!rows || !cols || !kwave || M < 1 || N < 1 || K < 32) return fail(BEAM_ERR_INVALID, "arguments");
+int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kind) {
+  if (!rows || !cols || !kind || M < 1 || N < 1 || K < 32) return fail(BEAM_ERR_INVALID, "arguments");
   const MxPlan plan = mx_plan(M, N, K, nullptr, false, g_dev.cus > 0 ? g_dev.cus : 256);
-  *rows = plan.rows, *cols = plan.cols, *kwave = plan.kwave;
+  *rows = plan.rows, *cols = plan.cols, *kind = plan.kind;
   return BEAM_OK;
 }
 

@@ -33,9 +33,9 @@ hipError_t launch_mx_kw(const MxParams& p, hipStream_t stream) {
 }  // namespace
 
 template <>
-hipError_t launch_gemm_mx<BEAM_T>(int block_m, int block_n, const MxParams& p, hipStream_t stream) {
-#define BEAM_MX(BM, BN, WVM, WVN, ST) \
-  if (block_m == BM && block_n == BN) return launch_mx_tile<BM, BN, WVM, WVN, ST>(p, stream);
+hipError_t launch_gemm_mx<BEAM_T>(int block_m, int block_n, int kind, const MxParams& p, hipStream_t stream) {
+#define BEAM_MX(BM, BN, KIND, WVM, WVN, ST) \
+  if (block_m == BM && block_n == BN && kind == KIND) return launch_mx_tile<BM, BN, WVM, WVN, ST>(p, stream);
   BEAM_FOR_EACH_MX_TILE(BEAM_MX)
 #undef BEAM_MX
   return hipErrorInvalidValue;

@@ -114,13 +114,18 @@ __device__ __forceinline__ i32x4 mx_encode_block(const V8 (&x)[4], int* scale) {
   return o;
 }
 
-// Launchers.  Tiles of MxGemm: (rows, columns, wavefronts along M and N, LDS slots); of MxKw: (rows, columns, wavefronts), those of 16
-// rows also with a16: p.A is 16-bit and K at most kMxKeptColumns.
-#define BEAM_FOR_EACH_MX_TILE(X) \
-  X(64, 64, 2, 2, 4)             \
-  X(128, 128, 2, 2, 4)           \
-  X(256, 128, 4, 2, 3)           \
-  X(256, 256, 2, 4, 2)
+// How an MXFP4 product runs: tiles of MxGemm, one workgroup to a CU or several of them with rings of fewer slots; of MxKw; of gemm_w4.h.
+enum MxKind : int { kMxAlone = 0, kMxKwave = 1, kMxWalk = 2, kMxShared = 3 };
+// Launchers.  Tiles of MxGemm: (rows, columns, kind, wavefronts along M and N, LDS slots); of MxKw: (rows, columns, wavefronts), those
+// of 16 rows also with a16: p.A is 16-bit and K at most kMxKeptColumns.
+#define BEAM_FOR_EACH_MX_TILE(X)    \
+  X(64, 64, kMxAlone, 2, 2, 4)      \
+  X(64, 64, kMxShared, 2, 2, 3)     \
+  X(128, 64, kMxShared, 4, 2, 3)    \
+  X(128, 128, kMxAlone, 4, 2, 4)    \
+  X(128, 128, kMxShared, 4, 2, 2)   \
+  X(256, 128, kMxAlone, 4, 2, 3)    \
+  X(256, 256, kMxAlone, 2, 4, 2)
 #define BEAM_FOR_EACH_MX_KWAVE(X) \
   X(16, 16, 4)                    \
   X(16, 32, 4)                    \
@@ -129,9 +134,9 @@ __device__ __forceinline__ i32x4 mx_encode_block(const V8 (&x)[4], int* scale) {
   X(32, 64, 4)                    \
   X(64, 32, 4)
 template <typename T>
-hipError_t launch_gemm_mx(int block_m, int block_n, const MxParams& p, hipStream_t stream);
-template <> hipError_t launch_gemm_mx<_Float16>(int, int, const MxParams&, hipStream_t);
-template <> hipError_t launch_gemm_mx<__bf16>(int, int, const MxParams&, hipStream_t);
+hipError_t launch_gemm_mx(int block_m, int block_n, int kind, const MxParams& p, hipStream_t stream);
+template <> hipError_t launch_gemm_mx<_Float16>(int, int, int, const MxParams&, hipStream_t);
+template <> hipError_t launch_gemm_mx<__bf16>(int, int, int, const MxParams&, hipStream_t);
 // The kernel of gemm_w4.h (256 x 256 tiles, a workgroup per CU walks them): K % 256 == 0, K >= 768, N % 8 == 0, C on 16 bytes.
 hipError_t launch_gemm_mx_w4(const MxW4Params& p, int dtype, dim3 grid, hipStream_t stream);
 template <typename T>

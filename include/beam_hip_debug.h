@@ -72,14 +72,14 @@ int beam_dbg_small_tile(int op, int M, int N, int K, int row_starts, int* rows, 
 /* Measurement only: the tile that MXFP4 products, and gated layers, run on from now on, named as beam_dbg_mx_tile and
  * beam_dbg_gated_tile name it, whether it is good for a problem or not; rows = 0: the library's choice again.  A tile that a problem
  * cannot run on is not taken, one that is not compiled makes the calls fail. */
-int beam_dbg_set_mx_tile(int rows, int cols, int kwave);
+int beam_dbg_set_mx_tile(int rows, int cols, int kind);
 int beam_dbg_set_gated_tile(int rows, int cols, int kind);
 /* ... and how the products of a gated layer's backward pass are cut into K slices, in tiles of rows (64, 128) x 128; slices = 1: not at
  * all; rows = -1: the library's choice again. */
 int beam_dbg_set_nn_split(int rows, int slices);
-/* What beam_gemmrc_mxfp4 runs an M x N x K problem on: a tile of rows x cols, *kwave 1 if its K tiles are dealt out to the wavefronts,
- * 2 if a workgroup on each CU walks the tiles (C on 16 bytes). */
-int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kwave);
+/* What beam_gemmrc_mxfp4 runs an M x N x K problem on: a tile of rows x cols, kind 0 a workgroup to a CU, 1 its K tiles are dealt out
+ * to the wavefronts, 2 a workgroup on each CU walks the tiles (C on 16 bytes), 3 several workgroups to a CU. */
+int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kind);
 /* What beam_gemmrc_gated runs an M x N x K problem on (K from 8 on): rows x cols rows of A and B, kind 0 tiles of gemm_kernel.h,
  * 1 tiles that a workgroup on each CU walks (outputs on 16 bytes), 2 the deep ones, 3 those that fill by whole lines, 4 tiles of
  * gemm_kwave.h, 5 those that fill by whole lines.  row_starts as in beam_dbg_small_tile. */

@@ -199,11 +199,14 @@ TILES = {
     (32, 32, 1): [(500, 493)],
     (32, 64, 1): [(500, 1003)],
     (64, 32, 1): [(9000, 20)],
-    (64, 64, 0): [(1000, 1001), (1024, 1024), (129, 9000)],
-    (128, 128, 0): [(200, 8531), (194, 8653)],
-    (256, 128, 0): [(515, 7513), (6673, 578)],
-    (256, 256, 0): [(835, 9511), (6303, 1283)],
-    (256, 256, 2): [(918, 8304), (4644, 1696), (8200, 4104)],
+    (64, 64, 0): [(135, 8316), (1433, 1383)],
+    (64, 64, 3): [(1000, 1001), (1024, 1024), (33, 8532)],
+    (128, 64, 3): [(68, 8403), (1080, 1100)],
+    (128, 128, 0): [(263, 9967), (1780, 1781)],
+    (128, 128, 3): [(409, 8215), (2060, 2070)],
+    (256, 128, 0): [(399, 8292), (2053, 2060)],
+    (256, 256, 0): [(1154, 7748), (7033, 1293)],
+    (256, 256, 2): [(944, 8416), (7714, 1040), (8200, 4104)],
 }
 
 
@@ -216,7 +219,7 @@ def tile_of(beamc, M, N, K):
 def test_problems_reach_the_tiles_that_they_are_listed_under(gpu, beamc):
     for tile, problems in TILES.items():
         for M, N in problems:
-            K = 4096 if tile[2] == 2 else 1024
+            K = 4096 if tile in ((256, 128, 0), (256, 256, 2)) else 1024
             assert tile_of(beamc, M, N, K) == tile, (M, N, tile_of(beamc, M, N, K))
 
 
