@@ -1017,7 +1017,8 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
 
 namespace {
 
-// The tile of gemm_kwave.h for a gated layer, if any; as kw_plan for its 2 N rows of B, of which the tiles here have 32 or 64.
+// The tile of gemm_kwave.h for a gated layer of which there is one for every CU at most, if any; as kw_plan for its 2 N rows of B, of
+// which the tiles here have 32 or 64.
 std::atomic<int> g_gated_rows{0}, g_gated_cols{0}, g_gated_kind{0};  // beam_dbg_set_gated_tile
 KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
   if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) {
@@ -1025,7 +1026,7 @@ KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
     const bool fits = K >= 8 && K <= kMaxK && (forced > 8 || M <= 8) && (kind == 4 || (kind == 5 && rows != kAnywhere && forced > 8));
     return fits ? KwPlan{forced, g_gated_cols.load(std::memory_order_relaxed), 4, kind == 5} : KwPlan{0, 0, 0, false};
   }
-  static const struct { int rows, cols; } kTiles[] = {{8, 32}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}, {64, 64}};
+  static const struct { int rows, cols; } kTiles[] = {{8, 32}, {16, 32}, {32, 32}, {16, 64}, {32, 64}, {64, 32}};
   const KwPlan none = {0, 0, 0, false};
   if (K < 8 || K > kMaxK) return none;
   for (const auto& t : kTiles) {
@@ -1036,35 +1037,69 @@ KwPlan gated_kw_plan(int M, int N, int K, RowStarts rows, int cus) {
     const bool few = M <= 16 && t.rows >= M && t.cols == 32;
     if (tiles > cus && !few) continue;
     const bool shift = rows == kOnChunks && t.rows > 8 && (long)(K / kBK) * (t.rows + t.cols) >= 1200;
-    if (t.rows * t.cols == 64 * 64 && (rows == kOnLines ? K >= 2048 : shift)) return none;
     return KwPlan{t.rows, t.cols, 4, shift};
   }
   return none;
 }
 
-// The tile of the gated kernel: what beam_gemmrc would take for the 2 N rows of B, as far as there is one like it.
-// walk_fits: the outputs are on 16 bytes.
+// The tile of the gated kernel for everything larger, by rounds of workgroups, each with a start and an end and its K tiles, which
+// take longer where rows start on 16 bytes only or anywhere (RowStarts); apart for a workgroup that has a CU to itself where two
+// would fit.  walk_fits: the outputs are on 16 bytes.
+// us, fitted to timings of every tile on 397 shapes (tokens 17 to 8192, N 64 to 14336, K 64 to 8192, with GU and without, on which the
+// choice does not depend): the picks are 0.5% behind the best tile on average and 19% at worst, 1043 x 7848 x 896 with GU; taking
+// what beam_gemmrc would was 3.4 and 36% (773 x 480 x 3272 18.3 -> 14.2 us, 3559 x 288 x 1152 15.7 -> 10.4, 3867 x 2356 x 3531 217 -> 183).  Each
+// is the best on some: those, for which all were timed, are 1375 x 256 x 192 4.6 in 64 x 64, 871 x 1024 x 3128 22.6 in 64 x 128 by lines
+// (25.4 in 96 x 128, 29.2 in 160 x 128), 485 x 1472 x 1024 7.8 in 64 x 128 deep (9.5 in 128 x 128 deep, 9.8 in 64 x 128), 1001 x 2001 x 2000
+// 21.5 in 160 x 128 (27.2 in 128 x 128 deep), 512 x 4096 x 1024 12.5 in 128 x 128 deep (15.3 in 128 x 128), 645 x 3776 x 424 11.9 in 256 x
+// 128 (14.6 in 128 x 128), 3572 x 5304 x 160 51.0 in 128 x 128 (63 in 256 x 256), 4096 x 14336 x 4096 644 walking (658 in 256 x 256, 738 in 224 x
+// 256), 2811 x 3792 x 361 41.5 in 224 x 256 (44.3 in 192 x 256), 998 x 8444 x 3435 181 in 192 x 256 (194 in 256 x 256, 204 in 256 x 128), 721 x
+// 2944 x 4544 49.4 in 160 x 128 (53.0 in 192 x 128), 960 x 2768 x 6336 73.2 in 192 x 128.
 GatedTile gated_tile(int M, int N, int K, RowStarts rows, bool walk_fits, int cus) {
   const bool walk = walk_fits && K % kBK == 0 && K >= kW4MinK && N % 8 == 0 && N <= (1 << 20) && (size_t)(N + 128) * K * 2 < ((size_t)1 << 31);
   if (const int forced = g_gated_rows.load(std::memory_order_relaxed)) {
     const int kind = g_gated_kind.load(std::memory_order_relaxed);
-    if ((kind != kGatedWalk || walk) && (kind != kGatedLines || rows != kAnywhere)) return GatedTile{forced, g_gated_cols.load(std::memory_order_relaxed), kind};
+    if (kind < kGatedKwave && (kind != kGatedWalk || walk) && (kind != kGatedLines || rows != kAnywhere))
+      return GatedTile{forced, g_gated_cols.load(std::memory_order_relaxed), kind};
   }
-  if (K % kBK != 0 && rows == kOnChunks) {
-    const LineChoice t = off_lines_tile(M, 2 * N, K, cus);
-    if (t.lines) return GatedTile{t.cfg.block_m == 128 && t.cfg.block_n == 64 ? 64 : t.cfg.block_m, 128, kGatedLines};
+  struct Cost {
+    double fixed, k_tile[3];  // by RowStarts: anywhere, on chunks, on lines
+  };
+  static const struct { GatedTile tile; int per_cu; Cost full, alone; } kTiles[] = {
+      {{64, 64, kGatedKwave}, 1, {2.8, {0.36, 0.27, 0.23}}, {}},
+      {{64, 64, kGatedKwaveLines}, 1, {3.95, {0, 0.21, 0.23}}, {}},
+      {{64, 128, kGatedShallow}, 2, {2.5, {0.99, 0.83, 0.66}}, {2.55, {0.71, 0.57, 0.49}}},
+      {{64, 128, kGatedDeep}, 1, {3.4, {0.53, 0.44, 0.35}}, {}},
+      {{64, 128, kGatedLines}, 1, {3.75, {0, 0.33, 0.35}}, {}},
+      {{96, 128, kGatedLines}, 1, {4.8, {0, 0.35, 0.42}}, {}},
+      {{128, 128, kGatedShallow}, 2, {3.5, {1.31, 1.18, 0.89}}, {3.35, {0.78, 0.69, 0.62}}},
+      {{128, 128, kGatedDeep}, 1, {4.1, {0.76, 0.59, 0.46}}, {}},
+      {{160, 128, kGatedLines}, 1, {4.8, {0, 0.51, 0.56}}, {}},
+      {{192, 128, kGatedLines}, 1, {7.5, {0, 0.53, 0.57}}, {}},
+      {{256, 128, kGatedShallow}, 1, {4.8, {1.08, 0.91, 0.76}}, {}},
+      {{192, 256, kGatedShallow}, 1, {6.4, {1.68, 1.18, 1.02}}, {}},
+      {{224, 256, kGatedShallow}, 1, {6.3, {1.69, 1.45, 1.12}}, {}},
+      {{256, 256, kGatedShallow}, 1, {9.5, {1.57, 1.32, 1.15}}, {}},
+      {{256, 256, kGatedWalk}, 1, {10.1, {0, 0, 1.11}}, {}},
+  };
+  const int k_tiles = (K + kBK - 1) / kBK;
+  GatedTile best = kTiles[2].tile;
+  double best_us = 1e300;
+  for (const auto& c : kTiles) {
+    if (c.full.k_tile[rows] == 0 || (c.tile.depth == kGatedWalk && !walk)) continue;
+    const long n = ((long)M + c.tile.block_m - 1) / c.tile.block_m * (((long)N + c.tile.block_n / 2 - 1) / (c.tile.block_n / 2)), slots = (long)cus * c.per_cu;
+    const bool alone = c.per_cu > 1 && n <= cus;
+    const double us = alone ? c.alone.fixed + c.alone.k_tile[rows] * k_tiles : (double)((n + slots - 1) / slots) * (c.full.fixed + c.full.k_tile[rows] * k_tiles);
+    if (us < best_us) best_us = us, best = c.tile;
   }
-  beam_tile_cfg c;
-  int s;
-  (void)choose_default(M, 2 * N, K, -1, &c, &s);
-  // From a round of workgroups on, the walking kernel, as in beam_gemmrc (choose_default names it by its wavefronts).
-  if (c.block_m == 256 && c.block_n == 256 && c.wave_m == 128 && c.wave_n == 128 && walk) return GatedTile{256, 256, kGatedWalk};
-  if (c.block_m * c.block_n <= 128 * 64) return GatedTile{64, 128, c.pipeline == 2 ? kGatedDeep : kGatedShallow};
-  // One 128 x 128 tile to a CU: its long ring, but for the shortest sums (512 x 4096 x 1024 16.8 -> 14.7 us, 1024 x 1024 x 1024 10.8 -> 9.6,
-  // 140 x 4480 x 448 7.8 -> 7.6; 603 x 2240 x 216 7.0, 7.4; 309 x 10816 x 128 5.9, 9.1).
-  const long tiles = (long)((M + 127) / 128) * ((N + 63) / 64);
-  if (c.block_m * c.block_n == 128 * 128 && (c.pipeline == 2 || (tiles <= cus && K >= 448))) return GatedTile{128, 128, kGatedDeep};
-  return GatedTile{c.block_m, c.block_n, kGatedShallow};
+  return best;
+}
+
+// What a gated layer runs on: a tile of gemm_kwave.h, if kw->rows is not 0, or *tile.
+void gated_plan(int M, int N, int K, RowStarts rows, bool walk_fits, int cus, KwPlan* kw, GatedTile* tile) {
+  *kw = gated_kw_plan(M, N, K, rows, cus);
+  if (kw->rows) return;
+  *tile = gated_tile(M, N, K, rows, walk_fits, cus);
+  if (tile->depth >= kGatedKwave) *kw = KwPlan{tile->block_m, tile->block_n, 4, tile->depth == kGatedKwaveLines};
 }
 
 // How a product of the backward pass, C [M][N] with B as [K][N], is cut into K slices; fewer than two: matmul_nn as it is.  What
@@ -1137,7 +1172,10 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
   }
   const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
   const RowStarts rows = row_starts(A, B, K, false);
-  if (const KwPlan kw = gated_kw_plan(M, N, K, rows, cus); kw.rows) {
+  KwPlan kw;
+  GatedTile t;
+  gated_plan(M, N, K, rows, (((uintptr_t)H | (uintptr_t)GU) & 15) == 0, cus, &kw, &t);
+  if (kw.rows) {
     KwGatedParams p;
     KwPlan half = kw;
     half.cols /= 2;
@@ -1146,7 +1184,6 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
     BEAM_HIP(dtype == BEAM_F16 ? launch_gated_kwave<_Float16>(kw, p, st) : launch_gated_kwave<__bf16>(kw, p, st));
     return BEAM_OK;
   }
-  const GatedTile t = gated_tile(M, N, K, rows, (((uintptr_t)H | (uintptr_t)GU) & 15) == 0, cus);
   const beam_tile_cfg c = {t.block_m, t.block_n / 2, 0, 0, 0, default_group_m(t.block_m, t.block_n)};
   GemmParams p = base_params(A, B, M, N, K, c);
   p.C = H;
@@ -2236,12 +2273,11 @@ int beam_dbg_mx_tile(int M, int N, int K, int* rows, int* cols, int* kind) {
 int beam_dbg_gated_tile(int M, int N, int K, int row_starts, int* rows, int* cols, int* kind) {
   if (!rows || !cols || !kind || row_starts < 0 || row_starts > 2) return fail(BEAM_ERR_INVALID, "arguments");
   const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
-  if (const KwPlan kw = gated_kw_plan(M, N, K, (RowStarts)row_starts, cus); kw.rows) {
-    *rows = kw.rows, *cols = kw.cols, *kind = kw.shift ? 5 : 4;
-    return BEAM_OK;
-  }
-  const GatedTile t = gated_tile(M, N, K, (RowStarts)row_starts, true, cus);
-  *rows = t.block_m, *cols = t.block_n, *kind = t.depth;
+  KwPlan kw;
+  GatedTile t;
+  gated_plan(M, N, K, (RowStarts)row_starts, true, cus, &kw, &t);
+  if (kw.rows) *rows = kw.rows, *cols = kw.cols, *kind = kw.shift ? kGatedKwaveLines : kGatedKwave;
+  else *rows = t.block_m, *cols = t.block_n, *kind = t.depth;
   return BEAM_OK;
 }
 

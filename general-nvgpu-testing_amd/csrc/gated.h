@@ -11,7 +11,8 @@
 namespace beam {
 
 // A workgroup tile of the gated kernel: block_n rows of B, half of them gate and half up rows, so block_n / 2 columns of C.
-enum GatedDepth : int { kGatedShallow = 0, kGatedWalk = 1, kGatedDeep = 2, kGatedLines = 3 };
+// (kGatedKwave, kGatedKwaveLines: the tile of that size of gemm_kwave.h, straight fills or whole lines.)
+enum GatedDepth : int { kGatedShallow = 0, kGatedWalk = 1, kGatedDeep = 2, kGatedLines = 3, kGatedKwave = 4, kGatedKwaveLines = 5 };
 struct GatedTile {
   int block_m, block_n, depth;
 };
@@ -22,7 +23,6 @@ struct GatedTile {
   X(224, 256, 2, 4, kGatedShallow, 3, 2, 1)      \
   X(192, 256, 2, 4, kGatedShallow, 3, 2, 1)      \
   X(256, 128, 4, 2, kGatedShallow, 3, 2, 1)      \
-  X(128, 256, 2, 4, kGatedShallow, 3, 2, 1)      \
   X(128, 128, 2, 2, kGatedShallow, 3, 2, 1)      \
   X(128, 128, 2, 2, kGatedDeep, 5, 4, 1)         \
   X(64, 128, 2, 2, kGatedShallow, 3, 2, 1)       \
@@ -31,7 +31,6 @@ struct GatedTile {
 #define BEAM_FOR_EACH_GATED_LINES_TILE(X)  \
   X(64, 128, 6, 2, kFormLineHalves)        \
   X(96, 128, 5, 2, kFormLineHalves)        \
-  X(128, 128, 5, 2, kFormLineHalves)       \
   X(160, 128, 4, 1, kFormLines)            \
   X(192, 128, 4, 2, kFormLineHalves)
 // Tiles of gemm_kwave.h: (rows, rows of B, wavefronts)

@@ -20,7 +20,7 @@ F16, BF16 = 0, 1
 HALF_STEP = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
 TINY = {F16: 2.0 ** -24, BF16: 2.0 ** -126}
 
-# (rows, rows of B, kind) of beam_dbg_gated_tile -> problems that it names
+# (rows, rows of B, kind) as in beam_dbg_gated_tile -> problems that are run on it
 TILES = {
     (8, 32, 4): [(1, 8, 9), (3, 70, 200), (8, 333, 64), (1, 1, 8), (1, 4135, 12), (5, 4267, 64)],
     (16, 32, 4): [(9, 9, 15), (16, 300, 513), (10, 8, 64), (10, 4365, 10), (9, 4447, 64), (16, 5000, 200)],
@@ -29,25 +29,54 @@ TILES = {
     (32, 64, 4): [(4627, 17, 9), (17, 4167, 8), (19, 4697, 64)],
     (64, 32, 4): [(4469, 39, 17), (4193, 37, 64)],
     (64, 64, 4): [(34, 4497, 17), (34, 4128, 8), (35, 4294, 64)],
+    (64, 64, 5): [(65, 2757, 1320)],
     (16, 32, 5): [(9, 9, 1736)],
     (16, 64, 5): [(37, 2125, 984)],
     (32, 32, 5): [(18, 2496, 1248)],
     (32, 64, 5): [(34, 2810, 992)],
     (64, 32, 5): [(926, 262, 840)],
     (64, 128, 0): [(70, 4112, 20), (69, 4297, 8), (83, 4097, 64)],
-    (64, 128, 2): [(147, 2903, 850), (340, 1377, 768)],
+    (64, 128, 2): [(68, 4226, 282), (147, 2903, 850), (340, 1377, 768)],
     (64, 128, 3): [(105, 4682, 480)],
-    (96, 128, 3): [(84, 4113, 424)],
+    (96, 128, 3): [(84, 4113, 424), (275, 1447, 1152)],
     (128, 128, 0): [(833, 2378, 22), (774, 2547, 8), (536, 3732, 64)],
-    (128, 128, 2): [(315, 3309, 1122), (715, 1380, 1152)],
-    (160, 128, 3): [(1390, 1489, 144)],
-    (192, 128, 3): [(544, 4260, 480)],
+    (128, 128, 2): [(1626, 611, 2404), (315, 3309, 1122), (715, 1380, 1152)],
+    (160, 128, 3): [(1390, 1489, 144), (1827, 1090, 72), (398, 4726, 256)],
+    (192, 128, 3): [(544, 4260, 480), (806, 1008, 960)],
     (192, 256, 0): [(4395, 948, 346), (1098, 3863, 344), (881, 4704, 384)],
     (224, 256, 0): [(1570, 3791, 122), (3592, 1699, 112), (2440, 2686, 128)],
     (256, 256, 0): [(3956, 1827, 164), (2246, 2957, 144), (2939, 2606, 192)],
     (256, 256, 1): [(1812, 3992, 192), (4096, 2048, 192), (3877, 1944, 192)],
     (256, 128, 0): [(1930, 1105, 1487), (1062, 2005, 1472)],
-    (128, 256, 0): [(1310, 2907, 2432)],
+}
+# ... -> problems that the library picks it for
+PICKED = {
+    (8, 32, 4): [(1, 4135, 12), (5, 4267, 64)],
+    (16, 32, 4): [(10, 8, 64), (9, 4447, 64)],
+    (16, 64, 4): [(40, 2700, 64), (37, 2125, 100)],
+    (32, 32, 4): [(4144, 8, 13), (31, 4000, 64)],
+    (32, 64, 4): [(4627, 17, 9), (17, 4167, 8), (19, 4697, 64)],
+    (64, 32, 4): [(4469, 39, 17), (4193, 37, 64)],
+    (16, 32, 5): [(9, 9, 1736)],
+    (16, 64, 5): [(37, 2125, 984)],
+    (32, 32, 5): [(18, 2496, 1248)],
+    (32, 64, 5): [(34, 2810, 992)],
+    (64, 32, 5): [(926, 262, 840)],
+    (64, 64, 4): [(33, 4223, 10), (34, 4215, 8), (33, 4144, 64)],
+    (64, 64, 5): [(34, 4216, 1360), (65, 2757, 1320)],
+    (64, 128, 0): [(68, 4166, 9), (72, 4141, 8), (65, 4125, 64)],
+    (64, 128, 2): [(68, 4226, 282), (69, 4102, 448)],
+    (64, 128, 3): [(65, 4241, 464)],
+    (96, 128, 3): [(4175, 194, 280), (275, 3447, 1152)],
+    (128, 128, 0): [(4763, 403, 10), (404, 4687, 8), (386, 4677, 64)],
+    (128, 128, 2): [(274, 3307, 2468), (4929, 261, 464), (4627, 195, 512)],
+    (160, 128, 3): [(1827, 1090, 72), (398, 4726, 256)],
+    (192, 128, 3): [(519, 4231, 480), (806, 3008, 960)],
+    (192, 256, 0): [(781, 4771, 721), (772, 5022, 8), (4353, 898, 64)],
+    (224, 256, 0): [(3935, 1035, 10), (1161, 4766, 8), (1190, 4723, 64)],
+    (256, 128, 0): [(529, 3678, 327), (495, 4103, 280), (485, 4627, 640)],
+    (256, 256, 0): [(4092, 1714, 130), (2033, 3252, 136), (1827, 3626, 256)],
+    (256, 256, 1): [(4096, 11008, 4096)],
 }
 
 
@@ -133,25 +162,31 @@ def run_forward(beamc, a, b, dtype, offsets=(0, 0, 0, 0), train=True):
     return h, (gu if train else None)
 
 
-def test_problems_reach_the_tiles_that_they_are_listed_under(gpu, beamc):
-    for tile, problems in TILES.items():
+def test_the_library_picks_every_tile(gpu, beamc):
+    assert set(PICKED) == set(TILES)
+    for tile, problems in PICKED.items():
         for M, N, K in problems:
             assert tile_of(beamc, M, N, K) == tile, (M, N, K)
 
 
 @pytest.mark.parametrize("tile", sorted(TILES), ids=lambda t: "x".join(map(str, t)))
 def test_forward(gpu, beamc, oracle, tile):
-    for i, (M, N, K) in enumerate(TILES[tile]):
-        dtype = (F16, BF16)[i % 2]
-        a, b = inputs(beamc, M, N, K, dtype)
-        h, gu = run_forward(beamc, a, b, dtype)
-        check_forward(oracle, a, b, h, gu, dtype, (tile, M, N, K, dtype))
-        again, _ = run_forward(beamc, a, b, dtype, train=False)
-        assert (again == h).all(), "h depends on whether gu is asked for"
-        other = 1 - dtype
-        a, b = inputs(beamc, M, N, K, other)
-        h, gu = run_forward(beamc, a, b, other, offsets=(1, 3, 8, 16) if tile[2] == 1 else (1, 3, 1, 5) if i % 2 else (8, 24, 2, 4))
-        check_forward(oracle, a, b, h, gu, other, (tile, M, N, K, other, "anywhere"))
+    beamc.lib.beam_dbg_set_gated_tile(*tile)
+    try:
+        for i, (M, N, K) in enumerate(TILES[tile]):
+            assert tile_of(beamc, M, N, K) == tile
+            dtype = (F16, BF16)[i % 2]
+            a, b = inputs(beamc, M, N, K, dtype)
+            h, gu = run_forward(beamc, a, b, dtype)
+            check_forward(oracle, a, b, h, gu, dtype, (tile, M, N, K, dtype))
+            again, _ = run_forward(beamc, a, b, dtype, train=False)
+            assert (again == h).all(), "h depends on whether gu is asked for"
+            other = 1 - dtype
+            a, b = inputs(beamc, M, N, K, other)
+            h, gu = run_forward(beamc, a, b, other, offsets=(1, 3, 8, 16) if tile[2] == 1 else (1, 3, 1, 5) if i % 2 else (8, 24, 2, 4))
+            check_forward(oracle, a, b, h, gu, other, (tile, M, N, K, other, "anywhere"))
+    finally:
+        beamc.lib.beam_dbg_set_gated_tile(0, 0, 0)
 
 
 @pytest.mark.parametrize("K", [1, 2, 7])
