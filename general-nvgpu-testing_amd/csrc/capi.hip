@@ -8,6 +8,7 @@
 #include <atomic>
 #include <chrono>
 #include <cstdlib>
+#include <initializer_list>
 #include <mutex>
 #include <set>
 #include <string>
@@ -1144,6 +1145,25 @@ int run_nn_split(const void* A, const void* B, void* C, int M, int N, int K, int
 }
 
 // A [M][K] and the layer's 2 N rows of B: what every entry refuses.
+// Bytes of memory that a call reads or writes; of the layers below what is written overlaps nothing else (a call whose output lies in
+// an operand would have workgroups read what others have written).
+struct Span {
+  const void* at;
+  size_t bytes;
+};
+int check_apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  auto meet = [](const Span& x, const Span& y) {
+    return x.at && y.at && (uintptr_t)x.at < (uintptr_t)y.at + y.bytes && (uintptr_t)y.at < (uintptr_t)x.at + x.bytes;
+  };
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span& r : read)
+      if (meet(*w, r)) return fail(BEAM_ERR_INVALID, "an output or the workspace overlaps an input");
+    for (const Span* o = w + 1; o != written.end(); ++o)
+      if (meet(*w, *o)) return fail(BEAM_ERR_INVALID, "outputs, or an output and the workspace, overlap");
+  }
+  return BEAM_OK;
+}
+
 int check_gated(const void* A, const void* B, const void* H, int M, int N, int K, int dtype, bool* generic) {
   if (N > INT32_MAX / 4) return fail(BEAM_ERR_UNSUPPORTED, "N=%d too large", N);
   return check_problem(A, B, H, M, N, K, dtype, generic);
@@ -1159,6 +1179,8 @@ int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, in
   if (rc) return rc;
   if ((uintptr_t)GU & 1) return fail(BEAM_ERR_INVALID, "GU must be aligned to its 16-bit elements");
   if (M == 0 || N == 0) return BEAM_OK;
+  const size_t mn = (size_t)M * N * 2;
+  if ((rc = check_apart({{H, mn}, {GU, 2 * mn}}, {{A, (size_t)M * K * 2}, {B, (size_t)N * K * 4}}))) return rc;
   if ((rc = beam_init())) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (K == 0) {
@@ -1236,6 +1258,8 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
   const size_t need = beam_gemmrc_gated_backward_workspace_bytes(M, N, K, dA != nullptr, dB != nullptr);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255) != 0))
     return fail(BEAM_ERR_WORKSPACE, "workspace of %zu bytes on 256 needed, %zu given", need, ws ? ws_bytes : (size_t)0);
+  const size_t mn = (size_t)M * N * 2, mk = (size_t)M * K * 2, nk = (size_t)N * K * 4;
+  if ((rc = check_apart({{dA, mk}, {dB, nk}, {ws, need}}, {{dH, mn}, {GU, 2 * mn}, {A, mk}, {B, nk}}))) return rc;
   if ((rc = beam_init())) return rc;
   char* const d = (char*)ws;
   char* const dt = d + (dA ? align_up((size_t)M * gated_line(2 * N) * 2, 256) : 0);
@@ -1268,6 +1292,9 @@ int check_mx(int rows, int K, int dtype) {
   if (((long)rows + 31) / 32 * (((long)K + kMxTile - 1) / kMxTile) > INT32_MAX) return fail(BEAM_ERR_UNSUPPORTED, "%d rows of K=%d are too many", rows, K);
   return BEAM_OK;
 }
+
+Span mx_elements(const void* elements, int rows, int K) { return {elements, (size_t)rows * (size_t)(K / 2)}; }
+Span mx_scales(const void* scales, int rows, int K) { return {scales, beam_mxfp4_scale_bytes(rows, K)}; }
 
 int check_mx_held(const void* elements, const void* scales, const char* what) {
   if (!elements || !scales) return fail(BEAM_ERR_INVALID, "null pointer to %s", what);
@@ -1389,7 +1416,8 @@ int beam_mxfp4_quantize(const void* X, void* elements, void* scales, int rows, i
   if (rc || rows == 0 || K == 0) return rc;
   if (!X) return fail(BEAM_ERR_INVALID, "null input pointer");
   if ((uintptr_t)X & 1) return fail(BEAM_ERR_INVALID, "X must be aligned to its 16-bit elements");
-  if ((rc = check_mx_held(elements, scales, "the result")) || (rc = beam_init())) return rc;
+  if ((rc = check_mx_held(elements, scales, "the result"))) return rc;
+  if ((rc = check_apart({mx_elements(elements, rows, K), mx_scales(scales, rows, K)}, {{X, (size_t)rows * K * 2}})) || (rc = beam_init())) return rc;
   BEAM_HIP(launch_mx_quantize(X, (uint8_t*)elements, (uint8_t*)scales, rows, K, dtype, (hipStream_t)stream));
   return BEAM_OK;
 }
@@ -1399,7 +1427,8 @@ int beam_mxfp4_dequantize(const void* elements, const void* scales, void* X, int
   if (rc || rows == 0 || K == 0) return rc;
   if (!X) return fail(BEAM_ERR_INVALID, "null output pointer");
   if ((uintptr_t)X & 1) return fail(BEAM_ERR_INVALID, "X must be aligned to its 16-bit elements");
-  if ((rc = check_mx_held(elements, scales, "the operand")) || (rc = beam_init())) return rc;
+  if ((rc = check_mx_held(elements, scales, "the operand"))) return rc;
+  if ((rc = check_apart({{X, (size_t)rows * K * 2}}, {mx_elements(elements, rows, K), mx_scales(scales, rows, K)})) || (rc = beam_init())) return rc;
   BEAM_HIP(launch_mx_dequantize((const uint8_t*)elements, (const uint8_t*)scales, X, rows, K, dtype, (hipStream_t)stream));
   return BEAM_OK;
 }
@@ -1409,6 +1438,7 @@ int beam_gemmrc_mxfp4(const void* A, const void* A_scales, const void* B, const 
   int rc = check_mx_product(C, M, N, K, dtype);
   if (rc || M == 0 || N == 0) return rc;
   if (K > 0 && ((rc = check_mx_held(A, A_scales, "A")) || (rc = check_mx_held(B, B_scales, "B")))) return rc;
+  if ((rc = check_apart({{C, (size_t)M * N * 2}}, {mx_elements(A, M, K), mx_scales(A_scales, M, K), mx_elements(B, N, K), mx_scales(B_scales, N, K)}))) return rc;
   if ((rc = beam_init())) return rc;
   if (K == 0) {
     BEAM_HIP(launch_zero_u16(C, (size_t)M * N, (hipStream_t)stream));
@@ -1433,6 +1463,7 @@ int beam_linear_mxfp4(const void* A, const void* B, const void* B_scales, void* 
   const size_t need = beam_linear_mxfp4_workspace_bytes(M, K);
   if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255) != 0))
     return fail(BEAM_ERR_WORKSPACE, "workspace of %zu bytes on 256 needed, %zu given", need, ws ? ws_bytes : (size_t)0);
+  if ((rc = check_apart({{C, (size_t)M * N * 2}, {ws, need}}, {{A, (size_t)M * K * 2}, mx_elements(B, N, K), mx_scales(B_scales, N, K)}))) return rc;
   if ((rc = beam_init())) return rc;
   if (need == 0) return run_mx(A, nullptr, true, B, B_scales, C, M, N, K, dtype, (hipStream_t)stream);
   char* const elements = (char*)ws;

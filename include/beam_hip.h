@@ -265,17 +265,17 @@ int beam_matmul_nn(const void* A, const void* B, void* C, int M, int N, int K, i
 /* H[M][N] = silu(G) * U with G = A . B[0..N)^T and U = A . B[N..2N)^T: B is [2N][K], the N rows of the gate's projection in front
  * of the N rows of the other one; both products, the activation and their product in one launch, from the fp32 sums, rounded
  * once.  GU, if not null: [M][2N], G and U rounded to the dtype, what the backward pass takes.  Any M, N, K and any element's
- * address.  H and GU must not overlap each other or an input.  No counterpart in the reference (its SiLU,
+ * address.  H and GU may not overlap each other or an input (refused).  No counterpart in the reference (its SiLU,
  * cuda/cute_kernels/cute_gemm_ln.cu:191-192, is a job beside a product). */
 int beam_gemmrc_gated(const void* A, const void* B, void* H, void* GU, int M, int N, int K, int dtype, void* stream);
 
 /* The gradients of that layer: with s = 1 / (1 + exp(-G)), D = [dH * U * s * (1 + G * (1 - s)), dH * G * s] ([M][2N], rounded to
  * the dtype for the products that follow: in fp16 infinite beyond 65504 and coarse below 2^-14, as any gradient held in fp16),
- * dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or dB may be null: not asked for; they overlap
- * neither each other nor an input.  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.  Three launches, and one more for a
- * product of so few outputs that its sums are cut into slices, which are added in their order; the workspace (256-byte
- * aligned, any contents) holds D, its transpose and such sums, and belongs to the call until it has run: calls that overlap in
- * time need one each, and so does a captured graph that may run beside another. */
+ * dA[M][K] = D . B and dB[2N][K] = D^T . A.  GU as beam_gemmrc_gated wrote it.  dA or dB may be null: not asked for; they may
+ * overlap neither each other nor an input nor the workspace (refused).  An empty sum (M = 0 for dB, N = 0 for dA) gives zeros.
+ * Three launches, and one more for a product of so few outputs that its sums are cut into slices, which are added in their
+ * order; the workspace (256-byte aligned, any contents) holds D, its transpose and such sums, and belongs to the call until it
+ * has run: calls that overlap in time need one each, and so does a captured graph that may run beside another. */
 size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int K, int want_dA, int want_dB);
 int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, const void* B, void* dA, void* dB, int M, int N, int K,
                                int dtype, void* ws, size_t ws_bytes, void* stream);
@@ -291,8 +291,8 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
 size_t beam_mxfp4_scale_bytes(int rows, int K);
 /* X [rows][K] (16-bit, any element's address) in that format: a block's power of two is the one at or below its largest magnitude,
  * over 4 (at least 2^-127); an element is the nearest value of the eight, ties to the even code, 6 beyond 6.  A block with an
- * infinity or a NaN in it gets the scale NaN, and is NaN in whatever is made of it.  Here and in the calls below, outputs overlap no
- * input. */
+ * infinity or a NaN in it gets the scale NaN, and is NaN in whatever is made of it.  Here and in the calls below, outputs that
+ * overlap an input or each other are refused. */
 int beam_mxfp4_quantize(const void* X, void* elements, void* scales, int rows, int K, int dtype, void* stream);
 /* The values held, in dtype (rounded to nearest where it cannot hold them). */
 int beam_mxfp4_dequantize(const void* elements, const void* scales, void* X, int rows, int K, int dtype, void* stream);

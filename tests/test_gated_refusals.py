@@ -27,6 +27,38 @@ def test_forward(beamc):
     refused(beamc, f(P, P, P, P, 1 << 30, 8, 8, F16, None), UNSUPPORTED, "too large")
 
 
+def test_overlaps(beamc):
+    """M 100, N 60, K 60: one byte of an output in something else."""
+    M, N, K = 100, 60, 60
+    sizes = {"a": M * K * 2, "b": N * K * 4, "h": M * N * 2, "gu": M * N * 4, "dh": M * N * 2, "da": M * K * 2, "db": N * K * 4}
+    ws_bytes = beamc.lib.beam_gemmrc_gated_backward_workspace_bytes(M, N, K, 1, 1)
+    sizes["ws"] = ws_bytes
+    apart, at = {}, P
+    for k, n in sizes.items():
+        apart[k] = at
+        at += (n + 511) // 256 * 256
+    last = {k: apart[k] + sizes[k] - 2 for k in sizes}
+
+    def forward(**kw):
+        v = {**apart, **kw}
+        return beamc.lib.beam_gemmrc_gated(v["a"], v["b"], v["h"], v["gu"], M, N, K, F16, None)
+
+    def backward(**kw):
+        v = {**apart, **kw}
+        return beamc.lib.beam_gemmrc_gated_backward(v["dh"], v["gu"], v["a"], v["b"], v["da"], v["db"], M, N, K, F16, v["ws"], ws_bytes, None)
+
+    for x in ("a", "b"):
+        for out in ("h", "gu"):
+            refused(beamc, forward(**{out: last[x]}), INVALID, "overlap")
+    refused(beamc, forward(h=last["gu"]), INVALID, "overlap")
+    for x in ("dh", "gu", "a", "b"):
+        for out in ("da", "db"):
+            refused(beamc, backward(**{out: last[x]}), INVALID, "overlap")
+        refused(beamc, backward(**{x: apart["ws"]}), INVALID, "overlap")
+    refused(beamc, backward(da=last["db"]), INVALID, "overlap")
+    refused(beamc, backward(da=last["ws"]), INVALID, "overlap")
+
+
 def test_backward(beamc):
     f, need = beamc.lib.beam_gemmrc_gated_backward, beamc.lib.beam_gemmrc_gated_backward_workspace_bytes
     n = need(100, 60, 8, 1, 1)

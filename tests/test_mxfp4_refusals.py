@@ -70,6 +70,41 @@ def test_products(beamc):
     refused(beamc, linear(bytes=need - 1), WORKSPACE, "workspace")
 
 
+def test_overlaps(beamc):
+    M, N, K = 100, 64, 64
+    need = beamc.lib.beam_linear_mxfp4_workspace_bytes(M, K)
+    sizes = {"x": M * K * 2, "a": M * K // 2, "sa": M * 8, "b": N * K // 2, "sb": N * 8, "c": M * N * 2, "ws": need}
+    apart, at = {}, P
+    for k, n in sizes.items():
+        apart[k] = at
+        at += (n + 511) // 256 * 256
+    back = {k: apart[k] + sizes[k] - 8 for k in sizes}  # on 8 bytes, the last of what is there
+    L = beamc.lib
+
+    def quantize(**kw):
+        v = {**apart, **kw}
+        return L.beam_mxfp4_quantize(v["x"], v["a"], v["sa"], M, K, F16, None)
+
+    def dequantize(**kw):
+        v = {**apart, **kw}
+        return L.beam_mxfp4_dequantize(v["a"], v["sa"], v["x"], M, K, F16, None)
+
+    def product(**kw):
+        v = {**apart, **kw}
+        return L.beam_gemmrc_mxfp4(v["a"], v["sa"], v["b"], v["sb"], v["c"], M, N, K, F16, None)
+
+    def linear(**kw):
+        v = {**apart, **kw}
+        return L.beam_linear_mxfp4(v["x"], v["b"], v["sb"], v["c"], M, N, K, F16, v["ws"], need, None)
+
+    for call, out, others in ((quantize, "sa", ("x", "a")), (dequantize, "x", ("a", "sa")), (product, "c", ("a", "sa", "b", "sb")),
+                              (linear, "c", ("x", "b", "sb", "ws"))):
+        for k in others:
+            refused(beamc, call(**{out: back[k]}), INVALID, "overlap")
+    for k in ("x", "b", "sb"):
+        refused(beamc, linear(**{k: apart["ws"]}), INVALID, "overlap")
+
+
 def test_python_layer(beamc):
     class Fake(beamc.DeviceArray):
         def __init__(self, shape, dtype=F16, itemsize=2):
