@@ -1106,13 +1106,14 @@ void gated_plan(int M, int N, int K, RowStarts rows, bool walk_fits, int cus, Kw
 // How a product of the backward pass, C [M][N] with B as [K][N], is cut into K slices; fewer than two: matmul_nn as it is.  What
 // slices save, a long sum on few CUs, has to pay for their partial sums and for a launch that adds them, 4 us and more: sums of
 // 4096 and more, on up to a third of the CUs.  us of the whole pass, without -> with (tokens x N x K): 16 x 11008 x 4096 139 -> 101,
-// 128 x 11008 x 4096 162 -> 116, 300 x 4096 x 1024 50 -> 36, 1024 x 2816 x 1024 58.7 -> 53.5; half the CUs 1001 x 2001 x 2000 67.7,
+// 128 x 11008 x 4096 162 -> 116, 300 x 4096 x 1024 50 -> 36, x 1025 56 -> 44, 1024 x 2816 x 1024 58.7 -> 53.5; half the CUs 1001 x 2001 x 2000 67.7,
 // 66.1; shorter sums 512 x 1024 x 512 17.0, 29.7; 1024 x 1024 x 1024 26.5, 31.4.
 struct NnSplit {
   int block_m, slices;
 };
 std::atomic<int> g_nn_split_rows{-1}, g_nn_split_slices{0};  // beam_dbg_set_nn_split
 NnSplit nn_split(int M, int N, int K, int cus) {
+  if (N < 8 || N > (N % 8 != 0 ? 1 << 23 : 1 << 24) || K > kMaxK) return NnSplit{64, 1};  // (matmul_nn's plain kernel)
   if (const int rows = g_nn_split_rows.load(std::memory_order_relaxed); rows >= 0) return NnSplit{rows, g_nn_split_slices.load(std::memory_order_relaxed)};
   const int rows = M <= 64 ? 64 : 128;
   const long tiles = (long)((M + rows - 1) / rows) * ((N + 127) / 128);
@@ -1144,7 +1145,6 @@ int run_nn_split(const void* A, const void* B, void* C, int M, int N, int K, int
   return BEAM_OK;
 }
 
-// A [M][K] and the layer's 2 N rows of B: what every entry refuses.
 // Bytes of memory that a call reads or writes; of the layers below what is written overlaps nothing else (a call whose output lies in
 // an operand would have workgroups read what others have written).
 struct Span {
@@ -1164,6 +1164,7 @@ int check_apart(std::initializer_list<Span> written, std::initializer_list<Span>
   return BEAM_OK;
 }
 
+// A [M][K] and the layer's 2 N rows of B: what every entry refuses.
 int check_gated(const void* A, const void* B, const void* H, int M, int N, int K, int dtype, bool* generic) {
   if (N > INT32_MAX / 4) return fail(BEAM_ERR_UNSUPPORTED, "N=%d too large", N);
   return check_problem(A, B, H, M, N, K, dtype, generic);
@@ -1232,15 +1233,17 @@ static size_t gated_operand_bytes(int M, int N, int want_dA, int want_dB) {
   return (want_dA ? align_up((size_t)M * gated_line(2 * N) * 2, 256) : 0) + (want_dB ? align_up((size_t)2 * N * gated_line(M) * 2, 256) : 0);
 }
 
-// Whether the products take rows of whole lines; then they may also be cut into slices.
+// Whether the products take rows of whole lines.
 static bool gated_lines(int M, int N, int K) { return K % 8 == 0 && K <= (1 << 23) && gated_line(2 * N) <= kMaxK && gated_line(M) <= kMaxK; }
 
 size_t beam_gemmrc_gated_backward_workspace_bytes(int M, int N, int K, int want_dA, int want_dB) {
   const size_t operands = gated_operand_bytes(M, N, want_dA, want_dB);
-  if (operands == 0 || K <= 0 || !gated_lines(M, N, K)) return operands;
+  if (operands == 0 || K <= 0) return operands;
   (void)beam_init();  // the number of slices depends on the device; a call on a host without one is refused there
   const int cus = g_dev.cus > 0 ? g_dev.cus : 256;
-  const size_t a = want_dA ? nn_split_bytes(M, K, gated_line(2 * N), cus) : 0, b = want_dB ? nn_split_bytes(2 * N, K, gated_line(M), cus) : 0;
+  const bool lines = gated_lines(M, N, K);
+  const size_t a = want_dA ? nn_split_bytes(M, K, lines ? gated_line(2 * N) : 2 * N, cus) : 0;
+  const size_t b = want_dB ? nn_split_bytes(2 * N, K, lines ? gated_line(M) : M, cus) : 0;
   return operands + (a > b ? a : b);  // one after the other
 }
 
@@ -1267,7 +1270,7 @@ int beam_gemmrc_gated_backward(const void* dH, const void* GU, const void* A, co
   char* const sums = d + gated_operand_bytes(M, N, dA != nullptr, dB != nullptr);
   const int cols_d = lines ? gated_line(2 * N) : 2 * N, cols_dt = lines ? gated_line(M) : M;
   if (M > 0 && N > 0) BEAM_HIP(launch_gated_gradients(dH, GU, dA ? d : nullptr, dB ? dt : nullptr, M, N, cols_d, cols_dt, dtype, (hipStream_t)stream));
-  if (!lines || M == 0 || N == 0) {
+  if (M == 0 || N == 0) {
     if (dA && (rc = matmul_nn(d, B, dA, M, K, cols_d, 2 * N, dtype, nullptr, stream))) return rc;
     return dB ? matmul_nn(dt, A, dB, 2 * N, K, cols_dt, M, dtype, nullptr, stream) : BEAM_OK;
   }

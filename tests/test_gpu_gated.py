@@ -419,7 +419,8 @@ def test_backward_of_infinities_in_the_last_row(gpu, beamc, oracle):
 
 
 @pytest.mark.parametrize("rows,slices", [(64, 2), (64, 7), (128, 3), (128, 16)])
-@pytest.mark.parametrize("M,N,K", [(1, 65, 8), (65, 63, 72), (200, 333, 136), (777, 256, 320), (1001, 501, 504)])
+@pytest.mark.parametrize("M,N,K", [(1, 65, 8), (65, 63, 72), (200, 333, 136), (777, 256, 320), (1001, 501, 504), (1, 65, 9), (65, 63, 75), (200, 333, 137),
+                                   (777, 256, 318), (1001, 501, 503), (129, 64, 12)])
 def test_backward_in_slices(gpu, beamc, oracle, rows, slices, M, N, K):
     """Sums cut into slices, whatever the problem: more than there are K tiles, and a last one that is short."""
     beamc.lib.beam_dbg_set_nn_split(rows, slices)
