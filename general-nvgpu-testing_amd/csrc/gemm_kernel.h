@@ -609,11 +609,11 @@ struct GemmTile {
     // this slice; anything else is out of range: reads return zero and touch no memory.
     int rows_a = (M - row0) < BM ? (M - row0) : BM;
     int rows_b = (N - col0) < CN ? (N - col0) : CN;
-    const size_t b_row0 = (size_t)col0 + (up_rows(lwave) ? (size_t)N : 0);
+    auto b_row0 = [&]() __attribute__((always_inline)) { return (size_t)col0 + (up_rows(lwave) ? (size_t)N : 0); };
     const T* a_base = (const T*)p.A + ((size_t)row0 * K + kb);
     // B as [N][K] (rows of K): like A.  B as [K][N] (B_KMAJOR): the tile's columns start at col0 of
     // row kb; a descriptor is made per K tile (load_b) so that it ends with the tile's last row.
-    const T* b_base = B_KMAJOR ? (const T*)p.B + ((size_t)kb * N + col0) : (const T*)p.B + (b_row0 * K + kb);
+    const T* b_base = B_KMAJOR ? (const T*)p.B + ((size_t)kb * N + col0) : (const T*)p.B + (b_row0() * K + kb);
     unsigned bytes_a = klen > 0 ? ((unsigned)(rows_a - 1) * K + klen) * 2u : 0u;  // (whole lines: chunks behind klen are masked)
     unsigned bytes_b = klen > 0 ? ((unsigned)(rows_b - 1) * K + klen) * 2u : 0u;
     // kEpiStoreLoop: the same for the next tile of this workgroup (neither split-K nor the [K][N]
@@ -782,7 +782,7 @@ struct GemmTile {
       };
       load_rows((const T*)p.A + (size_t)row0 * K, rows_a, std::integral_constant<int, LA>{}, st.a, [](int n) { return n; });
       if constexpr (!B_KMAJOR) {
-        load_rows((const T*)p.B + b_row0 * K, rows_b, std::integral_constant<int, LB>{}, st.b, [](int n) { return b_row(n); });
+        load_rows((const T*)p.B + b_row0() * K, rows_b, std::integral_constant<int, LB>{}, st.b, [](int n) { return b_row(n); });
       } else if (n_odd) {
         constexpr int CPR = BN / 8;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc((const T*)p.B + (size_t)koff * N, (unsigned)kvalid * (unsigned)N * 2u);
