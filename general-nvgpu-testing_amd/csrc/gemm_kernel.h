@@ -600,6 +600,7 @@ struct GemmTile {
       --kt_full;
     }
     const int n_all = kt_full + (k_tail ? 1 : 0);  // the short tile, if any, is tile 0
+    const int b_len = B_KMAJOR && p.b_rows - kb < klen ? p.b_rows - kb : klen;  // rows of B in this slice
     // Of this group.  Its tile t is tile t * GROUPS + kg of all; with lines a part of K in one piece, from k_first on.
     const int k_first = LINES && GROUPS > 1 ? kg * n_all / GROUPS : 0;
     const int n_tiles = GROUPS == 1 ? n_all : LINES ? (kg + 1) * n_all / GROUPS - k_first : (n_all - kg + GROUPS - 1) / GROUPS;
@@ -714,9 +715,8 @@ struct GemmTile {
         // columns past the last row's end are out of range and read as zeros.  (Columns past N in
         // earlier rows read the next row's data; they only feed output columns that do not exist.)
         const int koff = tile_koff(t);
-        int rows = klen - koff;
+        int rows = b_len - koff;
         if (rows > kBK) rows = kBK;
-        if (rows > p.b_rows - kb - koff) rows = p.b_rows - kb - koff;
         // (n_odd: another row of at least 8 elements follows every tile fetched here, so its last row may be read to a
         // whole chunk; the range check works on whole dwords and would cut an odd last column off)
         // (Whole lines: behind the last row that is multiplied here A's are zeros, and zero times infinity is not; one element
